@@ -140,6 +140,175 @@ lq8_status lq8_rms_norm_device(lq8_ctx* ctx, const float* d_x, const float* d_w,
 /* Tensor::silu, f32 branch (src/tensor.rs:1955-1990): x / (1 + exp(-x)). */
 lq8_status lq8_silu_device(lq8_ctx* ctx, const float* d_x, size_t n, float* d_y);
 
+/* ---- rotary positions with several axes --------------------------------------
+ * RotaryEmbedding (src/rope.rs:77-303) for positions that have more than one
+ * coordinate (time, height and width of a video patch), as device operators.
+ * Pairs p = 0 .. rotary_dim / 2 - 1 of a head: x[p] and x[p + rotary_dim / 2]
+ * turn by the angle
+ *   position[axis(p)] * theta^(-2 p / rotary_dim)
+ * (the angle is reduced in 64 bits, so a position of any int32 size keeps its
+ * digits); elements from rotary_dim on pass through.  axis(p):
+ *   LQ8_ROPE_SECTIONS     the first sections[0] pairs go by axis 0, the next
+ *                         sections[1] by axis 1, ...
+ *   LQ8_ROPE_INTERLEAVED  pair p goes by axis a = p % axes where a > 0 and
+ *                         p < axes * sections[a], else by axis 0
+ * Either way axis a has sections[a] pairs; they add up to rotary_dim / 2.
+ * With one axis all sections may be 0.
+ * repeated != 0: the reference's own frequencies, each used by two pairs
+ * (src/rope.rs:89-118): the exponent has p with its lowest bit cleared.
+ * head_dim and rotary_dim: multiples of 16, head_dim <= 256. */
+#define LQ8_ROPE_SECTIONS 0u
+#define LQ8_ROPE_INTERLEAVED 1u
+#define LQ8_ROPE_MAX_AXES 4
+typedef struct lq8_rope lq8_rope;
+typedef struct {
+    uint32_t head_dim, rotary_dim;
+    uint32_t axes;                          /* 1 .. LQ8_ROPE_MAX_AXES */
+    uint32_t sections[LQ8_ROPE_MAX_AXES];
+    uint32_t layout;                        /* LQ8_ROPE_SECTIONS or LQ8_ROPE_INTERLEAVED */
+    uint32_t repeated;
+    double theta;                           /* > 0 */
+} lq8_rope_config;
+/* Host-only: the checks of lq8_rope_create, and (axis_of_pair non-null) the
+ * axis of each of the rotary_dim / 2 pairs. */
+lq8_status lq8_rope_axes(const lq8_rope_config* cfg, uint8_t* axis_of_pair);
+lq8_status lq8_rope_create(lq8_ctx* ctx, const lq8_rope_config* cfg, lq8_rope** out);
+lq8_status lq8_rope_free(lq8_rope* rope);
+
+/* Rows to rotate: x and y of `dtype` (LQ8_DTYPE_F32 or LQ8_DTYPE_BF16),
+ * [rows][heads][head_dim], strides in elements from a row to the next (0:
+ * heads * head_dim).  y may be x itself (same stride); other overlaps are
+ * undefined.  positions: device int32 [axes][rows], positions_stride elements
+ * from an axis to the next (0: rows).  inverse: turns back (the transpose of
+ * the rotation, which is also its gradient; a cached key moved to another
+ * position).  Pointers and strides are multiples of 16 bytes. */
+typedef struct {
+    int32_t dtype;
+    uint32_t rows, heads, inverse;
+    const void* x;
+    void* y;
+    size_t x_stride, y_stride;
+    const int32_t* positions;
+    size_t positions_stride;
+} lq8_rope_rows;
+lq8_status lq8_rope_device(lq8_ctx* ctx, const lq8_rope* rope, const lq8_rope_rows* rows);
+
+/* ---- paged key/value cache -----------------------------------------------------
+ * KvCache (src/attention.rs:463-598) for a batch of sequences whose positions
+ * live in pages of one common allocation: position t of a sequence is slot
+ * t % page_size of page pages[t / page_size] of its table.  Keys and values
+ * are [num_pages][num_kv_heads][page_size][head_dim] of `dtype`
+ * (LQ8_DTYPE_F32 or LQ8_DTYPE_BF16), page_stride elements from a page to the
+ * next (0: num_kv_heads * page_size * head_dim; more, for instance, where a
+ * page holds all layers).  head_dim 64 or 128; page_size a power of two,
+ * 16 .. 1024.  Pointers and page_stride are multiples of 16 bytes. */
+typedef struct {
+    void* k;
+    void* v;
+    uint32_t num_pages, page_size, num_kv_heads, head_dim;
+    int32_t dtype;
+    size_t page_stride;
+} lq8_kv_pages;
+
+/* A ragged batch.  Sequence s has rows row_begin[s] .. row_begin[s + 1] - 1 of
+ * the row arrays (row_begin null: one row each, rows == batch), which are its
+ * last positions: with n rows and lengths[s] positions (the rows' own among
+ * them), row i is position lengths[s] - n + i.  A sequence may have no rows,
+ * or no positions.  row_begin, lengths and pages are device arrays that are
+ * read when the kernels run; the sizes here bound what they may say:
+ * `rows` rows in all, at most max_rows of one sequence (rows of a sequence
+ * past that are not worked on), max_pages table entries a sequence (positions
+ * past them do not exist).  A table entry outside [0, num_pages) holds
+ * nothing: its positions are not written and count as masked.  Rows from
+ * row_begin[batch] on are left as they were. */
+typedef struct {
+    uint32_t batch, rows, max_rows, max_pages;
+    const int32_t* row_begin; /* [batch + 1], ascending, or null */
+    const int32_t* lengths;   /* [batch] */
+    const int32_t* pages;     /* [batch][max_pages] */
+} lq8_paged_batch;
+
+/* The projections of the batch's rows: q [rows][num_heads][head_dim], k and v
+ * [rows][num_kv_heads][head_dim] of `dtype`, strides in elements from a row to
+ * the next (0: heads * head_dim).  They may be parts of one buffer.  q and
+ * q_out null: keys and values only.  q_out may be q (same stride).
+ * q_norm, k_norm (f32 [head_dim], null: none): RmsNorm::forward of each head
+ * before the rotation (src/attention.rs:350-358 with src/rms_norm.rs:143-176:
+ * input, weight and result rounded to bf16; the mean of squares in 64 bits).
+ * positions: device int32 [axes][rows] as lq8_rope_rows; null: a row's
+ * position in its sequence, on every axis. */
+typedef struct {
+    int32_t dtype;
+    uint32_t num_heads;
+    const void *q, *k, *v;
+    void* q_out;
+    size_t q_stride, k_stride, v_stride, q_out_stride;
+    const float *q_norm, *k_norm;
+    float eps;
+    const int32_t* positions;
+    size_t positions_stride;
+} lq8_qkv_rows;
+/* Attention::forward up to its KvCache::append (src/attention.rs:350-372,
+ * 507-559) for the rows of a batch: q and k normalised (optional) and rotated
+ * (rope null: not), q to q_out, k and v rounded to the cache's type (to
+ * nearest, ties to even) at their positions.  f32 rows go into f32 or bf16
+ * pages, bf16 rows into bf16 pages.  Two rows that name the same slot race.
+ * Enqueued without synchronizing. */
+lq8_status lq8_paged_append_device(lq8_ctx* ctx, const lq8_rope* rope, const lq8_kv_pages* kv,
+                                   const lq8_paged_batch* batch, const lq8_qkv_rows* rows);
+
+/* Queries and outputs of the batch's rows, [rows][num_heads][head_dim] of
+ * `dtype` (the pairs of types lq8_paged_append_device has).  num_heads a
+ * multiple of num_kv_heads: head h attends through kv head
+ * h / (num_heads / num_kv_heads).  out may be q (same stride).  scale: > 0. */
+typedef struct {
+    int32_t dtype;
+    uint32_t num_heads;
+    const void* q;
+    void* out;
+    size_t q_stride, out_stride;
+    float scale;
+} lq8_attn_rows;
+/* Attention::forward's softmax(scale q k^T) v (src/attention.rs:374-394) over
+ * the pages: the row at position p of its sequence sees positions 0 .. p.  A
+ * row that sees nothing gives zeros; what a row does not see never reaches it,
+ * whatever is stored there (NaN included).  Scores, maxima, sums and outputs
+ * are held in 32 bits; between f32 rows and their pages products are as exact
+ * as f32's, between bf16 ones the probabilities are rounded to bf16 before
+ * they meet the values.  A row's result depends on its own sequence and the
+ * sizes of the call, never on the other sequences.  Works in the context's
+ * scratch buffer; enqueued without synchronizing. */
+lq8_status lq8_paged_attention_device(lq8_ctx* ctx, const lq8_kv_pages* kv, const lq8_paged_batch* batch,
+                                      const lq8_attn_rows* rows);
+
+/* Prefixes that sequences of a batch share: sequences seq_begin[g] ..
+ * seq_begin[g + 1] - 1 have the lengths[g] positions in pages[g] before their
+ * own (lengths and pages of the batch count from there).  Device arrays; a
+ * sequence in no group has no prefix. */
+typedef struct {
+    uint32_t groups, max_pages;
+    const int32_t* seq_begin; /* [groups + 1], ascending */
+    const int32_t* lengths;   /* [groups] */
+    const int32_t* pages;     /* [groups][max_pages] */
+} lq8_shared_prefix;
+/* lq8_paged_attention_device where each row sees its group's whole prefix
+ * first: the prefix's keys and values are read once for all rows of the group
+ * instead of once a sequence. */
+lq8_status lq8_prefix_attention_device(lq8_ctx* ctx, const lq8_kv_pages* kv, const lq8_paged_batch* batch,
+                                       const lq8_shared_prefix* prefix, const lq8_attn_rows* rows);
+
+/* Host-only: the checks of the two calls above (prefix null: the first), and
+ * how they would run on num_workgroups compute units. */
+typedef struct {
+    uint32_t own_rows, own_splits;       /* rows (query row, head) a workgroup takes of a sequence; most pieces of its positions */
+    uint32_t own_chunk;                  /* positions of the shortest piece */
+    uint32_t prefix_rows, prefix_splits, prefix_chunk;
+    uint64_t workgroups;                 /* of the launches together, the joining one aside */
+    uint64_t scratch_bytes;              /* of the context's scratch buffer */
+} lq8_paged_info;
+lq8_status lq8_paged_plan(const lq8_kv_pages* kv, const lq8_paged_batch* batch, const lq8_shared_prefix* prefix,
+                          const lq8_attn_rows* rows, uint32_t num_workgroups, lq8_paged_info* out);
+
 /* ---- linear forward ------------------------------------------------------
  * Replaces: Linear::forward (src/attention.rs:101-136) and the 2-D
  * Tensor::matmul it calls (src/tensor.rs:804-817, 898-981, 2716-2753;

@@ -1,0 +1,529 @@
+// rope.hip -- rotary positions with several axes, and the append to a paged
+// key/value cache (gfx950).
+//
+// A pair (x[p], x[p + half]) turns by the angle position[axis(p)] * f_p.  The
+// table holds f_p / 2 pi in double: position * turns has 53 bits, so its
+// fraction is good to 2^-22 of a turn even at position 2^31 (a float32 angle
+// loses a radian there); the fraction is taken in double, reduced to an eighth
+// of a turn and handed to the float32 Taylor sums of sin and cos (the next
+// terms are below 3e-8 at pi / 4).
+//
+// A thread has 2 V elements of a head: V consecutive pairs, V = 16 bytes of
+// elements, or V from each half of what passes through.  head_dim / (2 V)
+// threads make a head, and a workgroup's threads go over the heads of one row
+// in steps that keep their pairs where that divides, so that the sines are
+// computed once a thread.
+#include <cmath>
+#include <new>
+
+#include "lq8_numerics.h"
+#include "paged.h"
+
+namespace lq8 {
+namespace {
+
+constexpr int RT = 256;  // threads of a workgroup
+
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+    static constexpr int V = 4;
+    static __device__ __forceinline__ void load(const void* p, float (&x)[4]) {
+        const float4 t = *(const float4*)p;
+        x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
+    }
+    static __device__ __forceinline__ void store(void* p, const float (&x)[4]) {
+        *(float4*)p = make_float4(x[0], x[1], x[2], x[3]);
+    }
+};
+
+// float -> bf16 to nearest, ties to even (NaN stays NaN), two to a word
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+    return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (__bf16)b) << 16);
+}
+template <> struct Vec<Bf16> {
+    static constexpr int V = 8;
+    static __device__ __forceinline__ void load(const void* p, float (&x)[8]) {
+        const uint4 t = *(const uint4*)p;
+        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+    static __device__ __forceinline__ void store(void* p, const float (&x)[8]) {
+        *(uint4*)p = make_uint4(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(x[4], x[5]), bf16_pair(x[6], x[7]));
+    }
+};
+
+// V values into a cache row of type C
+template <typename C, int V>
+__device__ __forceinline__ void store_cache(C* p, const float (&x)[V]) {
+    if constexpr (sizeof(C) == 4) {
+        *(float4*)p = make_float4(x[0], x[1], x[2], x[3]);
+    } else if constexpr (V == 4) {
+        *(uint2*)p = make_uint2(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]));
+    } else {
+        Vec<Bf16>::store(p, x);
+    }
+}
+
+// cos and sin of position * turns full circles
+__device__ __forceinline__ void turn(int position, double turns, float* c, float* s) {
+    const double t = (double)position * turns;
+    const double f = t - rint(t);      // -1/2 .. 1/2
+    const double k = rint(4.0 * f);    // the quarter, -2 .. 2
+    const float r = (float)((f - 0.25 * k) * 6.283185307179586477);
+    const float q = r * r;
+    float sn = fmaf(q, 2.7557319e-6f, -1.9841270e-4f);
+    sn = fmaf(q, sn, 8.3333333e-3f);
+    sn = fmaf(q, sn, -1.6666667e-1f);
+    sn = fmaf(r * q, sn, r);
+    float cs = fmaf(q, 2.4801587e-5f, -1.3888889e-3f);
+    cs = fmaf(q, cs, 4.1666667e-2f);
+    cs = fmaf(q, cs, -0.5f);
+    cs = fmaf(q, cs, 1.0f);
+    const int ki = (int)k;
+    const float a = ki & 1 ? sn : cs, b = ki & 1 ? cs : sn;  // |cos|, |sin| of the quarter
+    *c = ki == 1 || ki == 2 || ki == -2 ? -a : a;
+    *s = ki == -1 || ki == 2 || ki == -2 ? -b : b;
+}
+
+// What a thread does of a head: unit u holds pairs u V .. + V - 1 (elements at
+// lo and lo + half), or past the rotary part two runs of V elements.
+template <int V>
+struct Unit {
+    int lo, hi;
+    bool turns;
+    __device__ __forceinline__ Unit(int u, int half) {
+        turns = u * V < half;
+        lo = turns ? u * V : half + u * V;  // 2 half + (u V - half)
+        if (!turns) lo = 2 * half + 2 * (u * V - half);
+        hi = turns ? lo + half : lo + V;
+    }
+};
+
+template <int V>
+__device__ __forceinline__ void angles(const RopePair* table, int p0, const int32_t* positions, size_t stride, int row,
+                                       int fallback, bool inverse, float (&c)[V], float (&s)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const RopePair p = table[p0 + i];
+        const int at = positions ? positions[p.axis * stride + row] : fallback;
+        turn(at, p.turns, &c[i], &s[i]);
+        if (inverse) s[i] = -s[i];
+    }
+}
+
+template <int V>
+__device__ __forceinline__ void rotate(float (&a)[V], float (&b)[V], const float (&c)[V], const float (&s)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const float x = a[i], y = b[i];
+        a[i] = fmaf(x, c[i], -(y * s[i]));
+        b[i] = fmaf(y, c[i], x * s[i]);
+    }
+}
+
+struct RopeArgs {
+    const RopePair* table;
+    const char* x;
+    char* y;
+    size_t xs, ys;  // bytes
+    const int32_t* positions;
+    size_t ps;
+    int rows, heads, half, units, dim;
+    bool inverse;
+};
+
+template <typename T>
+__global__ __launch_bounds__(RT) void k_rope(RopeArgs a) {
+    constexpr int V = Vec<T>::V;
+    const int row = blockIdx.x, total = a.heads * a.units, step = gridDim.y * RT;
+    float c[V], s[V];
+    int have = -1;
+    for (int item = blockIdx.y * RT + threadIdx.x; item < total; item += step) {
+        const int h = item / a.units, u = item - h * a.units;
+        const Unit<V> w(u, a.half);
+        const size_t off = (size_t)h * a.dim * sizeof(T);
+        const char* x = a.x + row * a.xs + off;
+        char* y = a.y + row * a.ys + off;
+        float p[V], q[V];
+        Vec<T>::load(x + w.lo * sizeof(T), p);
+        Vec<T>::load(x + w.hi * sizeof(T), q);
+        if (w.turns) {
+            if (u != have) angles<V>(a.table, u * V, a.positions, a.ps, row, 0, a.inverse, c, s);
+            have = u;
+            rotate<V>(p, q, c, s);
+        }
+        Vec<T>::store(y + w.lo * sizeof(T), p);
+        Vec<T>::store(y + w.hi * sizeof(T), q);
+    }
+}
+
+struct AppendArgs {
+    PagesDev kv;
+    BatchDev batch;
+    const RopePair* table;  // null: no rotation
+    const char *q, *k, *v;  // q null: no queries
+    char* q_out;
+    size_t qs, ks, vs, qos;  // bytes
+    const float *q_norm, *k_norm;
+    float eps;
+    const int32_t* positions;
+    size_t ps;
+    int heads, half;
+};
+
+// The sequence of a row, by all threads of the workgroup; -1: none.
+__device__ __forceinline__ int sequence_of(const BatchDev& b, int row, int* first, int* count) {
+    if (!b.row_begin) {
+        *first = row, *count = 1;
+        return row;
+    }
+    __shared__ int found[3];
+    if (threadIdx.x == 0) found[0] = -1;
+    __syncthreads();
+    for (int s = threadIdx.x; s < b.batch; s += RT) {
+        const RowRange r = rows_of(b, s);
+        // at most one sequence of an ascending row_begin has the row
+        if (row >= r.first && row - r.first < r.count) found[0] = s, found[1] = r.first, found[2] = r.count;
+    }
+    __syncthreads();
+    *first = found[1], *count = found[2];
+    return found[0];
+}
+
+// x * rsqrt(mean(x^2) + eps) * w of a head whose LANES threads lie side by
+// side, x, w and the result rounded to bf16 (RmsNorm::forward); the squares
+// of bf16 values, their sum and the root in double, so that the one rounding
+// left is the result's own.
+template <int LANES, int V>
+__device__ __forceinline__ void norm_head(float (&a)[V], float (&b)[V], const float* w, const Unit<V>& u, float eps) {
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        a[i] = (float)(__bf16)a[i], b[i] = (float)(__bf16)b[i];
+        sum = fma((double)a[i], (double)a[i], sum);
+        sum = fma((double)b[i], (double)b[i], sum);
+    }
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d /= 2) sum += __shfl_xor(sum, d);
+    const double inv = 1.0 / sqrt(sum / (double)(2 * V * LANES) + (double)eps);
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        a[i] = (float)(__bf16)(float)((double)a[i] * inv * (double)(float)(__bf16)w[u.lo + i]);
+        b[i] = (float)(__bf16)(float)((double)b[i] * inv * (double)(float)(__bf16)w[u.hi + i]);
+    }
+}
+
+// One row of the batch: its q heads to q_out, its k and v heads to its slot.
+template <typename T, typename C, int D>
+__global__ __launch_bounds__(RT) void k_append(AppendArgs a) {
+    constexpr int V = Vec<T>::V, UNITS = D / (2 * V);
+    static_assert(RT % UNITS == 0 && 64 % UNITS == 0, "a head's threads lie in one wave");
+    const int row = blockIdx.x;
+    int first, count;
+    const int seq = sequence_of(a.batch, row, &first, &count);
+    if (seq < 0) return;  // no sequence has the row
+    const int64_t slot = (int64_t)a.batch.lengths[seq] - count + (row - first);
+    int page = -1;
+    if (slot >= 0 && slot < (int64_t)a.batch.max_pages << a.kv.page_shift)
+        page = a.batch.pages[(size_t)seq * a.batch.max_pages + (slot >> a.kv.page_shift)];
+    if (page >= a.kv.num_pages) page = -1;
+    const int in_page = (int)slot & ((1 << a.kv.page_shift) - 1);
+    const int qh = a.q ? a.heads : 0, total = (qh + 2 * a.kv.kv_heads) * UNITS;
+    const int u = threadIdx.x % UNITS;
+    const Unit<V> w(u, a.half);
+    float c[V], s[V];
+    if (a.table && w.turns) angles<V>(a.table, u * V, a.positions, a.ps, row, (int)slot, false, c, s);
+    for (int item = blockIdx.y * RT + threadIdx.x; item < total; item += gridDim.y * RT) {
+        const int h = item / UNITS;  // whole heads: RT is a multiple of UNITS, so is total
+        const bool isq = h < qh, isk = !isq && h < qh + a.kv.kv_heads;
+        const int g = isq ? h : isk ? h - qh : h - qh - a.kv.kv_heads;
+        const char* src = (isq ? a.q + row * a.qs : isk ? a.k + row * a.ks : a.v + row * a.vs) + (size_t)g * D * sizeof(T);
+        float p[V], q[V];
+        Vec<T>::load(src + w.lo * sizeof(T), p);
+        Vec<T>::load(src + w.hi * sizeof(T), q);
+        if (isq || isk) {
+            const float* nw = isq ? a.q_norm : a.k_norm;
+            if (nw) norm_head<UNITS, V>(p, q, nw, w, a.eps);
+            if (a.table && w.turns) rotate<V>(p, q, c, s);
+        }
+        if (isq) {
+            char* y = a.q_out + row * a.qos + (size_t)g * D * sizeof(T);
+            Vec<T>::store(y + w.lo * sizeof(T), p);
+            Vec<T>::store(y + w.hi * sizeof(T), q);
+        } else if (page >= 0) {
+            C* y = (C*)(isk ? a.kv.k : a.kv.v) + page * a.kv.page_stride + (((size_t)g << a.kv.page_shift) + in_page) * D;
+            store_cache<C, V>(y + w.lo, p);
+            store_cache<C, V>(y + w.hi, q);
+        }
+    }
+}
+
+// Workgroups that share a row's heads: so many that about two a CU run.
+unsigned head_parts(size_t rows, size_t items, int cus) {
+    const size_t most = (items + RT - 1) / RT, want = (2 * (size_t)cus + rows - 1) / rows;
+    return (unsigned)(want < most ? want : most);
+}
+
+template <typename T, typename C>
+void launch_append(const AppendArgs& a, dim3 grid, int dim, hipStream_t s) {
+    if (dim == 64) hipLaunchKernelGGL((k_append<T, C, 64>), grid, dim3(RT), 0, s, a);
+    else hipLaunchKernelGGL((k_append<T, C, 128>), grid, dim3(RT), 0, s, a);
+}
+
+lq8_status check_rope(const lq8_rope_config* c) {
+    if (!c) return fail(LQ8_ERR_INVALID_ARG, "rope: null configuration");
+    if (c->head_dim == 0 || c->head_dim % 16 || c->head_dim > 256)
+        return fail(LQ8_ERR_SHAPE_MISMATCH, "rope: head_dim must be a multiple of 16 up to 256");
+    if (c->rotary_dim == 0 || c->rotary_dim % 16 || c->rotary_dim > c->head_dim)
+        return fail(LQ8_ERR_SHAPE_MISMATCH, "rope: rotary_dim must be a multiple of 16 up to head_dim");
+    if (c->axes < 1 || c->axes > LQ8_ROPE_MAX_AXES) return fail(LQ8_ERR_INVALID_ARG, "rope: 1 to 4 axes");
+    if (c->layout != LQ8_ROPE_SECTIONS && c->layout != LQ8_ROPE_INTERLEAVED)
+        return fail(LQ8_ERR_INVALID_ARG, "rope: unknown layout");
+    if (!(c->theta > 0.0) || !std::isfinite(c->theta)) return fail(LQ8_ERR_INVALID_ARG, "rope: theta must be positive");
+    const uint32_t pairs = c->rotary_dim / 2;
+    uint64_t sum = 0;
+    for (uint32_t a = 0; a < c->axes; a++) sum += c->sections[a];
+    if (!(c->axes == 1 && sum == 0) && sum != pairs)
+        return fail(LQ8_ERR_SHAPE_MISMATCH, "rope: the sections must add up to rotary_dim / 2");
+    if (c->layout == LQ8_ROPE_INTERLEAVED)
+        for (uint32_t a = 1; a < c->axes; a++)
+            if (c->sections[a] && (uint64_t)c->axes * (c->sections[a] - 1) + a >= pairs)
+                return fail(LQ8_ERR_SHAPE_MISMATCH, "rope: an interleaved section reaches past the last pair");
+    return LQ8_OK;
+}
+
+int axis_of(const lq8_rope_config& c, uint32_t p) {
+    if (c.axes == 1) return 0;
+    if (c.layout == LQ8_ROPE_INTERLEAVED) {
+        const uint32_t a = p % c.axes;
+        return a > 0 && p < (uint64_t)c.axes * c.sections[a] ? (int)a : 0;
+    }
+    uint32_t end = 0;
+    for (uint32_t a = 0; a + 1 < c.axes; a++) {
+        end += c.sections[a];
+        if (p < end) return (int)a;
+    }
+    return (int)c.axes - 1;
+}
+
+size_t elem_size(int32_t dtype) { return dtype == LQ8_DTYPE_F32 ? 4 : 2; }
+
+}  // namespace
+
+// ---- host checks ------------------------------------------------------------------
+
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+lq8_status check_pages(const lq8_kv_pages* kv, PagesDev* out) {
+    if (!kv) return fail(LQ8_ERR_INVALID_ARG, "pages: null description");
+    if (!kv->k || !kv->v) return fail(LQ8_ERR_INVALID_ARG, "pages: null pointer");
+    if (kv->dtype != LQ8_DTYPE_F32 && kv->dtype != LQ8_DTYPE_BF16)
+        return fail(LQ8_ERR_DTYPE_MISMATCH, "pages: F32 or BF16");
+    if (kv->head_dim != 64 && kv->head_dim != 128) return fail(LQ8_ERR_SHAPE_MISMATCH, "pages: head_dim must be 64 or 128");
+    if (kv->page_size < (uint32_t)PAGE_MIN || kv->page_size > (uint32_t)PAGE_MAX || (kv->page_size & (kv->page_size - 1)))
+        return fail(LQ8_ERR_SHAPE_MISMATCH, "pages: page_size must be a power of two from 16 to 1024");
+    if (kv->num_kv_heads == 0 || kv->num_kv_heads > MAX_KV_HEADS)
+        return fail(LQ8_ERR_SHAPE_MISMATCH, "pages: 1 to 1024 kv heads");
+    if (kv->num_pages == 0 || kv->num_pages > (uint32_t)INT32_MAX) return fail(LQ8_ERR_SHAPE_MISMATCH, "pages: no pages, or too many");
+    const size_t dense = (size_t)kv->num_kv_heads * kv->page_size * kv->head_dim, es = elem_size(kv->dtype);
+    const size_t stride = kv->page_stride ? kv->page_stride : dense;
+    if (stride < dense) return fail(LQ8_ERR_SHAPE_MISMATCH, "pages: page_stride is below a page");
+    if (stride > ((size_t)1 << 60) / kv->num_pages) return fail(LQ8_ERR_SHAPE_MISMATCH, "pages: page_stride too large");
+    if (!aligned16(kv->k) || !aligned16(kv->v) || (stride * es) % 16)
+        return fail(LQ8_ERR_INVALID_ARG, "pages: pointers and page_stride must be multiples of 16 bytes");
+    out->k = kv->k;
+    out->v = kv->v;
+    out->num_pages = (int)kv->num_pages;
+    out->page_shift = __builtin_ctz(kv->page_size);
+    out->kv_heads = (int)kv->num_kv_heads;
+    out->page_stride = stride;
+    return LQ8_OK;
+}
+
+lq8_status check_batch(const lq8_paged_batch* b, uint32_t page_size, BatchDev* out) {
+    if (!b) return fail(LQ8_ERR_INVALID_ARG, "batch: null description");
+    if (b->batch > MAX_BATCH || b->rows > MAX_ROWS) return fail(LQ8_ERR_SHAPE_MISMATCH, "batch: above 65536 sequences or 2^24 rows");
+    if (b->batch && b->rows) {
+        if (!b->lengths || !b->pages) return fail(LQ8_ERR_INVALID_ARG, "batch: null pointer");
+        if (!b->row_begin && b->rows != b->batch)
+            return fail(LQ8_ERR_SHAPE_MISMATCH, "batch: without row_begin every sequence has one row");
+        if (b->row_begin && (b->max_rows == 0 || b->max_rows > b->rows))
+            return fail(LQ8_ERR_SHAPE_MISMATCH, "batch: max_rows must be from 1 to rows");
+        if (b->max_pages == 0 || (uint64_t)b->max_pages * page_size > (uint64_t)INT32_MAX / 2)
+            return fail(LQ8_ERR_SHAPE_MISMATCH, "batch: max_pages is zero or holds more than 2^30 positions");
+    }
+    out->batch = (int)b->batch;
+    out->rows = (int)b->rows;
+    out->max_rows = b->row_begin ? (int)b->max_rows : 1;
+    out->max_pages = (int)b->max_pages;
+    out->row_begin = b->row_begin;
+    out->lengths = b->lengths;
+    out->pages = b->pages;
+    return LQ8_OK;
+}
+
+lq8_status check_types(int32_t rows, int32_t pages, PagedTypes* out) {
+    if (rows == LQ8_DTYPE_F32 && pages == LQ8_DTYPE_F32) *out = PT_F32_F32;
+    else if (rows == LQ8_DTYPE_F32 && pages == LQ8_DTYPE_BF16) *out = PT_F32_BF16;
+    else if (rows == LQ8_DTYPE_BF16 && pages == LQ8_DTYPE_BF16) *out = PT_BF16_BF16;
+    else return fail(LQ8_ERR_DTYPE_MISMATCH, "rows and pages: F32 with F32 or BF16 pages, BF16 with BF16 pages");
+    return LQ8_OK;
+}
+
+lq8_status check_rows(const char* what, const void* p, size_t* stride, size_t width, size_t elem) {
+    if (!p) return fail(LQ8_ERR_INVALID_ARG, std::string(what) + ": null pointer");
+    if (*stride == 0) *stride = width;
+    if (*stride < width || *stride > (size_t)1 << 32) return fail(LQ8_ERR_SHAPE_MISMATCH, std::string(what) + ": stride below a row, or above 2^32");
+    if (!aligned16(p) || (*stride * elem) % 16)
+        return fail(LQ8_ERR_INVALID_ARG, std::string(what) + ": pointer and stride must be multiples of 16 bytes");
+    return LQ8_OK;
+}
+
+}  // namespace lq8
+
+using namespace lq8;
+
+#define CHECK_CTX(ctx) \
+    if (!registry_has(ctx)) return fail(LQ8_ERR_INVALID_ARG, "invalid or released context handle")
+
+// positions of every axis lie inside what the strides span
+static lq8_status check_positions(const int32_t* p, size_t* stride, size_t rows) {
+    if (!p) return LQ8_OK;
+    if (*stride == 0) *stride = rows;
+    if (*stride < rows || *stride > (size_t)1 << 32) return fail(LQ8_ERR_SHAPE_MISMATCH, "positions: stride below the rows, or above 2^32");
+    return LQ8_OK;
+}
+
+extern "C" {
+
+lq8_status lq8_rope_axes(const lq8_rope_config* cfg, uint8_t* axis_of_pair) {
+    const lq8_status st = check_rope(cfg);
+    if (st) return st;
+    if (axis_of_pair)
+        for (uint32_t p = 0; p < cfg->rotary_dim / 2; p++) axis_of_pair[p] = (uint8_t)axis_of(*cfg, p);
+    return LQ8_OK;
+}
+
+lq8_status lq8_rope_create(lq8_ctx* ctx, const lq8_rope_config* cfg, lq8_rope** out) {
+    lq8_status st = check_rope(cfg);
+    if (st) return st;
+    CHECK_CTX(ctx);
+    if (!out) return fail(LQ8_ERR_INVALID_ARG, "out is null");
+    *out = nullptr;
+    DeviceGuard guard(ctx->device);
+    if (guard.status) return guard.status;
+    RopePair host[128];
+    const uint32_t pairs = cfg->rotary_dim / 2;
+    for (uint32_t p = 0; p < pairs; p++) {
+        const double e = -2.0 * (double)(cfg->repeated ? p & ~1u : p) / (double)cfg->rotary_dim;
+        host[p] = {std::pow(cfg->theta, e) / 6.283185307179586477, axis_of(*cfg, p), 0};
+    }
+    lq8_rope* r = new (std::nothrow) lq8_rope();
+    if (!r) return fail(LQ8_ERR_OUT_OF_MEMORY, "rope: host memory");
+    r->device = ctx->device;
+    r->cfg = *cfg;
+    hipError_t e = hipMalloc(&r->table, pairs * sizeof(RopePair));
+    if (e == hipSuccess) e = hipMemcpyAsync(r->table, host, pairs * sizeof(RopePair), hipMemcpyHostToDevice, ctx->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+    if (e != hipSuccess) {
+        if (r->table) (void)hipFree(r->table);
+        delete r;
+        return hip_fail(e, "rope table");
+    }
+    registry_add(r);
+    *out = r;
+    return LQ8_OK;
+}
+
+lq8_status lq8_rope_free(lq8_rope* rope) {
+    if (!registry_has(rope)) return fail(LQ8_ERR_INVALID_ARG, "invalid or released rope handle");
+    // (the context may be gone; hipFree waits for the table's readers)
+    registry_remove(rope);
+    (void)hipFree(rope->table);
+    delete rope;
+    return LQ8_OK;
+}
+
+lq8_status lq8_rope_device(lq8_ctx* ctx, const lq8_rope* rope, const lq8_rope_rows* rows) {
+    CHECK_CTX(ctx);
+    if (!registry_has(rope)) return fail(LQ8_ERR_INVALID_ARG, "invalid or released rope handle");
+    if (!rows) return fail(LQ8_ERR_INVALID_ARG, "rope: null rows");
+    if (rope->device != ctx->device) return fail(LQ8_ERR_INVALID_ARG, "rope: the handle is another device's");
+    if (rows->dtype != LQ8_DTYPE_F32 && rows->dtype != LQ8_DTYPE_BF16) return fail(LQ8_ERR_DTYPE_MISMATCH, "rope: F32 or BF16 rows");
+    if (rows->rows > MAX_ROWS || rows->heads > MAX_HEADS) return fail(LQ8_ERR_SHAPE_MISMATCH, "rope: above 2^24 rows or 16384 heads");
+    if (rows->rows == 0 || rows->heads == 0) return LQ8_OK;
+    const size_t es = elem_size(rows->dtype), width = (size_t)rows->heads * rope->cfg.head_dim;
+    size_t xs = rows->x_stride, ys = rows->y_stride, ps = rows->positions_stride;
+    lq8_status st;
+    if ((st = check_rows("rope x", rows->x, &xs, width, es)) || (st = check_rows("rope y", rows->y, &ys, width, es))) return st;
+    if (rows->x == rows->y && xs != ys) return fail(LQ8_ERR_SHAPE_MISMATCH, "rope: in place needs one stride");
+    if (!rows->positions) return fail(LQ8_ERR_INVALID_ARG, "rope: null positions");
+    if ((st = check_positions(rows->positions, &ps, rows->rows))) return st;
+    DeviceGuard guard(ctx->device);
+    if (guard.status) return guard.status;
+    const bool f32 = rows->dtype == LQ8_DTYPE_F32;
+    const int units = (int)rope->cfg.head_dim / (2 * (f32 ? 4 : 8));
+    RopeArgs a{(const RopePair*)rope->table, (const char*)rows->x, (char*)rows->y, xs * es, ys * es, rows->positions, ps,
+               (int)rows->rows, (int)rows->heads, (int)rope->cfg.rotary_dim / 2, units, (int)rope->cfg.head_dim,
+               rows->inverse != 0};
+    const dim3 grid(rows->rows, head_parts(rows->rows, (size_t)rows->heads * units, ctx->num_cus));
+    if (f32) hipLaunchKernelGGL(k_rope<float>, grid, dim3(RT), 0, ctx->stream, a);
+    else hipLaunchKernelGGL(k_rope<Bf16>, grid, dim3(RT), 0, ctx->stream, a);
+    LQ8_HIP(hipGetLastError());
+    return LQ8_OK;
+}
+
+lq8_status lq8_paged_append_device(lq8_ctx* ctx, const lq8_rope* rope, const lq8_kv_pages* kv,
+                                   const lq8_paged_batch* batch, const lq8_qkv_rows* rows) {
+    AppendArgs a{};
+    PagedTypes types;
+    lq8_status st;
+    if ((st = check_pages(kv, &a.kv)) || (st = check_batch(batch, kv->page_size, &a.batch))) return st;
+    if (!rows) return fail(LQ8_ERR_INVALID_ARG, "append: null rows");
+    if ((st = check_types(rows->dtype, kv->dtype, &types))) return st;
+    if (!rows->q != !rows->q_out) return fail(LQ8_ERR_INVALID_ARG, "append: q and q_out go together");
+    if (rows->q && (rows->num_heads == 0 || rows->num_heads > MAX_HEADS))
+        return fail(LQ8_ERR_SHAPE_MISMATCH, "append: 1 to 16384 query heads");
+    const size_t es = elem_size(rows->dtype), d = kv->head_dim;
+    size_t qs = rows->q_stride, ks = rows->k_stride, vs = rows->v_stride, os = rows->q_out_stride, ps = rows->positions_stride;
+    if ((st = check_rows("append k", rows->k, &ks, kv->num_kv_heads * d, es)) ||
+        (st = check_rows("append v", rows->v, &vs, kv->num_kv_heads * d, es)))
+        return st;
+    if (rows->q) {
+        if ((st = check_rows("append q", rows->q, &qs, rows->num_heads * d, es)) ||
+            (st = check_rows("append q_out", rows->q_out, &os, rows->num_heads * d, es)))
+            return st;
+        if (rows->q == rows->q_out && qs != os) return fail(LQ8_ERR_SHAPE_MISMATCH, "append: q in place needs one stride");
+    }
+    if ((rows->q_norm || rows->k_norm) && !(rows->eps >= 0.0f)) return fail(LQ8_ERR_INVALID_ARG, "append: eps must be at least 0");
+    if ((st = check_positions(rows->positions, &ps, batch->rows))) return st;
+    CHECK_CTX(ctx);
+    if (rope) {
+        if (!registry_has(rope)) return fail(LQ8_ERR_INVALID_ARG, "invalid or released rope handle");
+        if (rope->device != ctx->device) return fail(LQ8_ERR_INVALID_ARG, "append: the rope handle is another device's");
+        if (rope->cfg.head_dim != kv->head_dim) return fail(LQ8_ERR_SHAPE_MISMATCH, "append: rope of another head_dim");
+    }
+    if (batch->batch == 0 || batch->rows == 0) return LQ8_OK;
+    DeviceGuard guard(ctx->device);
+    if (guard.status) return guard.status;
+    a.table = rope ? (const RopePair*)rope->table : nullptr;
+    a.half = rope ? (int)rope->cfg.rotary_dim / 2 : (int)d / 2;
+    a.q = (const char*)rows->q, a.k = (const char*)rows->k, a.v = (const char*)rows->v, a.q_out = (char*)rows->q_out;
+    a.qs = qs * es, a.ks = ks * es, a.vs = vs * es, a.qos = os * es;
+    a.q_norm = rows->q_norm, a.k_norm = rows->k_norm, a.eps = rows->eps;
+    a.positions = rows->positions, a.ps = ps;
+    a.heads = rows->q ? (int)rows->num_heads : 0;
+    const size_t units = d / (2 * (rows->dtype == LQ8_DTYPE_F32 ? 4 : 8));
+    const dim3 grid(batch->rows, head_parts(batch->rows, (a.heads + 2 * (size_t)kv->num_kv_heads) * units, ctx->num_cus));
+    if (types == PT_F32_F32) launch_append<float, float>(a, grid, (int)d, ctx->stream);
+    else if (types == PT_F32_BF16) launch_append<float, Bf16>(a, grid, (int)d, ctx->stream);
+    else launch_append<Bf16, Bf16>(a, grid, (int)d, ctx->stream);
+    LQ8_HIP(hipGetLastError());
+    return LQ8_OK;
+}
+
+}  // extern "C"

@@ -114,6 +114,52 @@ class SamplingC(C.Structure):
                 ("repetition_penalty", C.c_float), ("seed", C.c_uint64)]
 
 
+class RopeConfigC(C.Structure):
+    _fields_ = [("head_dim", C.c_uint32), ("rotary_dim", C.c_uint32), ("axes", C.c_uint32),
+                ("sections", C.c_uint32 * 4), ("layout", C.c_uint32), ("repeated", C.c_uint32), ("theta", C.c_double)]
+
+
+class RopeRowsC(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("rows", C.c_uint32), ("heads", C.c_uint32), ("inverse", C.c_uint32),
+                ("x", C.c_void_p), ("y", C.c_void_p), ("x_stride", C.c_size_t), ("y_stride", C.c_size_t),
+                ("positions", C.c_void_p), ("positions_stride", C.c_size_t)]
+
+
+class KVPagesC(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("num_pages", C.c_uint32), ("page_size", C.c_uint32),
+                ("num_kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("dtype", C.c_int32),
+                ("page_stride", C.c_size_t)]
+
+
+class PagedBatchC(C.Structure):
+    _fields_ = [("batch", C.c_uint32), ("rows", C.c_uint32), ("max_rows", C.c_uint32), ("max_pages", C.c_uint32),
+                ("row_begin", C.c_void_p), ("lengths", C.c_void_p), ("pages", C.c_void_p)]
+
+
+class QkvRowsC(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("num_heads", C.c_uint32), ("q", C.c_void_p), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("q_out", C.c_void_p), ("q_stride", C.c_size_t), ("k_stride", C.c_size_t),
+                ("v_stride", C.c_size_t), ("q_out_stride", C.c_size_t), ("q_norm", C.c_void_p),
+                ("k_norm", C.c_void_p), ("eps", C.c_float), ("positions", C.c_void_p),
+                ("positions_stride", C.c_size_t)]
+
+
+class AttnRowsC(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("num_heads", C.c_uint32), ("q", C.c_void_p), ("out", C.c_void_p),
+                ("q_stride", C.c_size_t), ("out_stride", C.c_size_t), ("scale", C.c_float)]
+
+
+class SharedPrefixC(C.Structure):
+    _fields_ = [("groups", C.c_uint32), ("max_pages", C.c_uint32), ("seq_begin", C.c_void_p),
+                ("lengths", C.c_void_p), ("pages", C.c_void_p)]
+
+
+class PagedInfoC(C.Structure):
+    _fields_ = [("own_rows", C.c_uint32), ("own_splits", C.c_uint32), ("own_chunk", C.c_uint32),
+                ("prefix_rows", C.c_uint32), ("prefix_splits", C.c_uint32), ("prefix_chunk", C.c_uint32),
+                ("workgroups", C.c_uint64), ("scratch_bytes", C.c_uint64)]
+
+
 # lq8_generate_ex flag: the reference's generate() loop as written
 GEN_FEED_FIRST_TOKEN = 1
 # lq8_quantize_activations_device sources
@@ -205,6 +251,19 @@ _SIGS = [
     ("lq8_moe_routing", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     ("lq8_moe_clear_kv_cache", C.c_int, [C.c_void_p]),
     ("lq8_moe_free", C.c_int, [C.c_void_p]),
+    ("lq8_rope_axes", C.c_int, [C.POINTER(RopeConfigC), C.c_void_p]),
+    ("lq8_rope_create", C.c_int, [C.c_void_p, C.POINTER(RopeConfigC), C.POINTER(C.c_void_p)]),
+    ("lq8_rope_free", C.c_int, [C.c_void_p]),
+    ("lq8_rope_device", C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(RopeRowsC)]),
+    ("lq8_paged_append_device", C.c_int,
+     [C.c_void_p, C.c_void_p, C.POINTER(KVPagesC), C.POINTER(PagedBatchC), C.POINTER(QkvRowsC)]),
+    ("lq8_paged_attention_device", C.c_int,
+     [C.c_void_p, C.POINTER(KVPagesC), C.POINTER(PagedBatchC), C.POINTER(AttnRowsC)]),
+    ("lq8_prefix_attention_device", C.c_int,
+     [C.c_void_p, C.POINTER(KVPagesC), C.POINTER(PagedBatchC), C.POINTER(SharedPrefixC), C.POINTER(AttnRowsC)]),
+    ("lq8_paged_plan", C.c_int,
+     [C.POINTER(KVPagesC), C.POINTER(PagedBatchC), C.POINTER(SharedPrefixC), C.POINTER(AttnRowsC), C.c_uint32,
+      C.POINTER(PagedInfoC)]),
 ]
 
 EXPORTED = [s[0] for s in _SIGS]
@@ -723,6 +782,185 @@ def sample_device(ctx: Context, logits: "DeviceBuffer", vocab: int, config: Gene
         return int(tok.download(np.uint32, 1)[0])
     finally:
         tok.free()
+
+
+# ---- rotary positions and the paged key/value cache --------------------------------
+#
+# Each description below holds the structure of include/lq8.h with its device
+# pointers (any object with a ``ptr``: DeviceBuffer, or a wrapped tensor) and
+# keeps those objects alive.  A serving loop makes them once and calls the
+# operators with them step after step; only what the device arrays say changes.
+
+ROPE_SECTIONS, ROPE_INTERLEAVED = 0, 1
+
+
+def _dev(b):
+    return None if b is None else b.ptr
+
+
+def rope_config(head_dim: int, theta: float, rotary_dim: Optional[int] = None, sections: Sequence[int] = (),
+                interleaved: bool = False, repeated: bool = False) -> RopeConfigC:
+    """lq8_rope_config: sections[a] pairs turn with axis a's positions (none:
+    one axis); repeated: the reference's frequencies (src/rope.rs:89-118)."""
+    if len(sections) > 4:
+        raise InvalidArgument("rope: 1 to 4 axes")
+    sec = (C.c_uint32 * 4)(*sections)
+    return RopeConfigC(head_dim, head_dim if rotary_dim is None else rotary_dim, max(1, len(sections)), sec,
+                       ROPE_INTERLEAVED if interleaved else ROPE_SECTIONS, int(repeated), theta)
+
+
+def rope_axes(cfg: RopeConfigC) -> np.ndarray:
+    """The axis of each pair (lq8_rope_axes; no device)."""
+    out = np.zeros(max(1, min(cfg.rotary_dim, 256) // 2), dtype=np.uint8)
+    _check(lib().lq8_rope_axes(C.byref(cfg), _ptr(out)))
+    return out
+
+
+class Rope:
+    """Rotary frequencies of one to four position axes on the device
+    (RotaryEmbedding, src/rope.rs:77-303); see rope_config."""
+
+    def __init__(self, ctx: Context, head_dim: int, theta: float, rotary_dim: Optional[int] = None,
+                 sections: Sequence[int] = (), interleaved: bool = False, repeated: bool = False):
+        self.ctx, self.handle = ctx, None
+        self.cfg = rope_config(head_dim, theta, rotary_dim, sections, interleaved, repeated)
+        h = C.c_void_p()
+        _check(lib().lq8_rope_create(ctx.handle, C.byref(self.cfg), C.byref(h)))
+        self.handle = h
+
+    def free(self) -> None:
+        if self.handle:
+            _check(lib().lq8_rope_free(self.handle))
+            self.handle = None
+
+
+class RopeRows:
+    """Rows x [rows][heads][head_dim] to rotate into y (lq8_rope_rows)."""
+
+    def __init__(self, x, y, rows: int, heads: int, head_dim: int, positions, dtype: int = DTYPE_F32, x_stride: int = 0,
+                 y_stride: int = 0, positions_stride: int = 0, inverse: bool = False):
+        self.keep, self.head_dim = (x, y, positions), head_dim
+        self.c = RopeRowsC(dtype, rows, heads, int(inverse), _dev(x), _dev(y), x_stride, y_stride, _dev(positions),
+                           positions_stride)
+
+
+def rope_device(ctx: Context, rope: Rope, rows: RopeRows) -> None:
+    """RotaryEmbedding::apply (src/rope.rs:167-219) over device rows."""
+    if rows.head_dim != rope.cfg.head_dim:
+        raise ShapeMismatch(f"rows of head_dim {rows.head_dim}, rope of {rope.cfg.head_dim}")
+    _check(lib().lq8_rope_device(ctx.handle, rope.handle, rows.c))
+
+
+class KVPages:
+    """Pages of keys and values [num_pages][num_kv_heads][page_size][head_dim]
+    (lq8_kv_pages)."""
+
+    def __init__(self, k, v, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, dtype: int = DTYPE_F32,
+                 page_stride: int = 0):
+        self.keep, self.owned = (k, v), ()
+        self.c = KVPagesC(_dev(k), _dev(v), num_pages, page_size, num_kv_heads, head_dim, dtype, page_stride)
+
+    @classmethod
+    def alloc(cls, ctx: Context, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
+              dtype: int = DTYPE_F32) -> "KVPages":
+        """Pages of its own (not cleared); free() gives them back."""
+        nbytes = num_pages * num_kv_heads * page_size * head_dim * (4 if dtype == DTYPE_F32 else 2)
+        k = DeviceBuffer(ctx, nbytes)
+        try:
+            v = DeviceBuffer(ctx, nbytes)
+        except LludaError:
+            k.free()
+            raise
+        pages = cls(k, v, num_pages, page_size, num_kv_heads, head_dim, dtype)
+        pages.owned = (k, v)
+        return pages
+
+    def free(self) -> None:
+        for b in self.owned:
+            b.free()
+        self.owned = ()
+
+
+class PagedBatch:
+    """A ragged batch over a paged cache (lq8_paged_batch): device int32
+    arrays lengths [batch], pages [batch][max_pages] and, unless every sequence
+    has one row, row_begin [batch + 1]."""
+
+    def __init__(self, lengths, pages, batch: int, max_pages: int, rows: Optional[int] = None, row_begin=None,
+                 max_rows: int = 1):
+        self.keep = (lengths, pages, row_begin)
+        self.c = PagedBatchC(batch, batch if rows is None else rows, max_rows, max_pages, _dev(row_begin), _dev(lengths),
+                             _dev(pages))
+
+
+class QkvRows:
+    """The projections of a batch's rows (lq8_qkv_rows); stride: the row stride
+    of q, k and v alike (0: each its own width)."""
+
+    def __init__(self, q, k, v, num_heads: int, head_dim: int, q_out=None, stride: int = 0, q_out_stride: int = 0,
+                 q_norm=None, k_norm=None, eps: float = 1e-6, positions=None, positions_stride: int = 0,
+                 dtype: int = DTYPE_F32):
+        self.keep, self.head_dim = (q, k, v, q_out, q_norm, k_norm, positions), head_dim
+        self.c = QkvRowsC(dtype, num_heads, _dev(q), _dev(k), _dev(v), _dev(q_out), stride, stride, stride, q_out_stride,
+                          _dev(q_norm), _dev(k_norm), eps, _dev(positions), positions_stride)
+
+
+class AttnRows:
+    """Queries and outputs of a batch's rows (lq8_attn_rows); scale None:
+    1 / sqrt(head_dim)."""
+
+    def __init__(self, q, out, num_heads: int, head_dim: int, dtype: int = DTYPE_F32, q_stride: int = 0,
+                 out_stride: int = 0, scale: Optional[float] = None):
+        self.keep, self.head_dim = (q, out), head_dim
+        self.c = AttnRowsC(dtype, num_heads, _dev(q), _dev(out), q_stride, out_stride,
+                           head_dim ** -0.5 if scale is None else scale)
+
+
+class SharedPrefix:
+    """Prefixes that groups of a batch's sequences share (lq8_shared_prefix):
+    device int32 arrays seq_begin [groups + 1], lengths [groups], pages
+    [groups][max_pages]."""
+
+    def __init__(self, seq_begin, lengths, pages, groups: int, max_pages: int):
+        self.keep = (seq_begin, lengths, pages)
+        self.c = SharedPrefixC(groups, max_pages, _dev(seq_begin), _dev(lengths), _dev(pages))
+
+
+def _same_dim(kv: KVPages, rows) -> None:
+    if rows.head_dim != kv.c.head_dim:
+        raise ShapeMismatch(f"rows of head_dim {rows.head_dim}, pages of {kv.c.head_dim}")
+
+
+def paged_append_device(ctx: Context, rope: Optional[Rope], kv: KVPages, batch: PagedBatch, rows: QkvRows) -> None:
+    """Normalise and rotate q and k, write k and v into the pages
+    (lq8_paged_append_device; KvCache::append, src/attention.rs:507-559)."""
+    _same_dim(kv, rows)
+    _check(lib().lq8_paged_append_device(ctx.handle, rope.handle if rope is not None else None, kv.c, batch.c, rows.c))
+
+
+def paged_attention_device(ctx: Context, kv: KVPages, batch: PagedBatch, rows: AttnRows) -> None:
+    """softmax(scale q k^T) v over the pages (lq8_paged_attention_device;
+    src/attention.rs:374-394)."""
+    _same_dim(kv, rows)
+    _check(lib().lq8_paged_attention_device(ctx.handle, kv.c, batch.c, rows.c))
+
+
+def prefix_attention_device(ctx: Context, kv: KVPages, batch: PagedBatch, prefix: SharedPrefix, rows: AttnRows) -> None:
+    """paged_attention_device behind the groups' shared prefixes
+    (lq8_prefix_attention_device)."""
+    _same_dim(kv, rows)
+    _check(lib().lq8_prefix_attention_device(ctx.handle, kv.c, batch.c, prefix.c, rows.c))
+
+
+def paged_plan(kv: KVPages, batch: PagedBatch, rows: AttnRows, prefix: Optional[SharedPrefix] = None,
+               num_workgroups: int = 256) -> dict:
+    """lq8_paged_plan: the checks of the attention calls and how they would
+    run.  No device."""
+    _same_dim(kv, rows)
+    info = PagedInfoC()
+    _check(lib().lq8_paged_plan(kv.c, batch.c, prefix.c if prefix is not None else None, rows.c, num_workgroups,
+                                C.byref(info)))
+    return {n: int(getattr(info, n)) for n, _ in PagedInfoC._fields_}
 
 
 # ---- Qwen3-MoE decoder layers --------------------------------------------------
