@@ -21,7 +21,9 @@ struct RopePair {
 };
 
 constexpr int PAGE_MIN = 16, PAGE_MAX = 1024;
-constexpr uint32_t MAX_KV_HEADS = 1024, MAX_HEADS = 16384, MAX_BATCH = 65536, MAX_ROWS = 1u << 24;
+constexpr uint32_t MAX_KV_HEADS = 1024, MAX_HEADS = 16384, MAX_BATCH = 65536;
+// a launch has at most 2^32 threads: 256 of a row, 64 of a row's head
+constexpr uint32_t MAX_ROWS = 1u << 23, MAX_ROW_HEADS = 1u << 25;
 
 // Element types of a call: rows in T, pages in C.
 enum PagedTypes : int { PT_F32_F32 = 0, PT_F32_BF16 = 1, PT_BF16_BF16 = 2 };
@@ -37,15 +39,16 @@ struct BatchDev {
     const int32_t *row_begin, *lengths, *pages;
 };
 
-// Rows of sequence s, inside [0, rows] whatever row_begin says.
+// Rows of sequence s, inside [0, rows] whatever row_begin says: `total` of
+// them, of which the first `count` are worked on (max_rows).
 struct RowRange {
-    int first, count;
+    int first, total, count;
 };
 __device__ __forceinline__ RowRange rows_of(const BatchDev& b, int s) {
-    if (!b.row_begin) return {s, 1};
+    if (!b.row_begin) return {s, 1, 1};
     const int lo = min(max(b.row_begin[s], 0), b.rows);
     const int hi = min(max(b.row_begin[s + 1], lo), b.rows);
-    return {lo, min(hi - lo, b.max_rows)};
+    return {lo, hi - lo, min(hi - lo, b.max_rows)};
 }
 
 // Positions of a table with `length` of them that can exist.

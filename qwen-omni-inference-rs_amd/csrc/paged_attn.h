@@ -1,0 +1,151 @@
+// paged_attn.h -- what the kernels of attention over a paged cache share
+// (paged_few.hip, paged_tile.hip, paged_attention.hip).
+//
+// Rows.  The queries of a kv head are packed: packed row r of a sequence (or
+// of a group's rows) is query head r % G of row r / G, G = num_heads /
+// num_kv_heads.  Row i of a sequence sees positions 0 .. base + i - 1.
+//
+// Pieces.  A long row range of positions is cut into pieces that run on
+// different workgroups: piece c holds positions c * len .. of its sequence,
+// len from the sequence's own length alone (piece_len), so that a row's bits do
+// not depend on its batch.  A piece gives (o, m, l) per row: m the largest
+// scaled score in units of log 2, o = sum 2^(s - m) v, l = sum 2^(s - m).
+// m = -inf: the row sees nothing of it; m = -FLT_MAX: it does, and every score
+// is -inf.  With one piece, and no prefix, the kernel writes o / l itself.
+#pragma once
+
+#include <cfloat>
+
+#include "lq8_numerics.h"
+#include "paged.h"
+
+namespace lq8 {
+
+struct PrefixDev {
+    int groups = 0, max_pages = 0;
+    const int32_t *seq_begin = nullptr, *lengths = nullptr, *pages = nullptr;
+};
+
+struct Cut {
+    int pieces = 1;     // at most
+    int shortest = 64;  // positions of the shortest piece, a multiple of the kernel's tile
+    int unit = 64;      // pieces are multiples of it
+};
+
+struct AttnArgs {
+    PagesDev kv;
+    BatchDev batch;
+    PrefixDev prefix;
+    const char* q;
+    char* out;
+    size_t qs, os;  // elements
+    int heads, group;
+    float c;        // scale * log2(e)
+    Cut own, pre;
+    float* part;    // [slots][rows][heads][head_dim], own pieces first; null: one piece, results go to out
+    float2* ml;     // [slots][rows][heads]
+};
+
+__host__ __device__ inline int piece_len(int length, const Cut& c) {
+    const int n0 = (length + c.shortest - 1) / c.shortest;
+    const int n = n0 < c.pieces ? (n0 < 1 ? 1 : n0) : c.pieces;
+    const int len = (length + n - 1) / n;
+    return len < 1 ? c.unit : (len + c.unit - 1) / c.unit * c.unit;
+}
+
+// What one workgroup's rows attend to.
+struct Span {
+    int first, total, count;  // rows
+    const int32_t* table;
+    int length;               // positions that exist
+    int base;                 // row i sees min(max(base + i, 0), length)
+    __device__ __forceinline__ int sees(int i) const { return min(max(base + i, 0), length); }
+};
+__device__ __forceinline__ Span own_span(const AttnArgs& a, int s) {
+    const RowRange r = rows_of(a.batch, s);
+    const int raw = max(a.batch.lengths[s], 0);
+    return {r.first, r.total, r.count, a.batch.pages + (size_t)s * a.batch.max_pages,
+            held(raw, a.batch.max_pages, a.kv.page_shift), raw - r.total + 1};
+}
+// rows of the sequences of group g, each of which sees the whole prefix
+__device__ __forceinline__ Span prefix_span(const AttnArgs& a, int g) {
+    const int b = min(max(a.prefix.seq_begin[g], 0), a.batch.batch);
+    const int e = min(max(a.prefix.seq_begin[g + 1], b), a.batch.batch);
+    const int lo = !a.batch.row_begin ? b : min(max(a.batch.row_begin[b], 0), a.batch.rows);
+    const int hi = !a.batch.row_begin ? e : min(max(a.batch.row_begin[e], lo), a.batch.rows);
+    return {lo, hi - lo, hi - lo, a.prefix.pages + (size_t)g * a.prefix.max_pages,
+            held(a.prefix.lengths[g], a.prefix.max_pages, a.kv.page_shift), 1 << 30};
+}
+
+// The page of position j, -1 where none holds it.
+__device__ __forceinline__ int page_at(const AttnArgs& a, const Span& s, int j, int end) {
+    if (j >= end) return -1;
+    const int p = s.table[j >> a.kv.page_shift];
+    return (unsigned)p < (unsigned)a.kv.num_pages ? p : -1;
+}
+// Element offset of position j (in page p) of kv head g; p < 0: of the cache's first slots, which are there to be read.
+__device__ __forceinline__ size_t slot_off(const AttnArgs& a, int p, int g, int j, int dim) {
+    return p < 0 ? 0 : p * a.kv.page_stride + (((size_t)g << a.kv.page_shift) + (j & ((1 << a.kv.page_shift) - 1))) * dim;
+}
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (__bf16)b) << 16);
+}
+__device__ __forceinline__ float low_bf16(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high_bf16(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+
+// x = t[0] + t[1] + t[2] with terms of bf16, exactly: 8 + 8 + 8 bits.  The
+// first is cut, not rounded (a rounded one could be infinite); what is not
+// finite is its own first term.
+__device__ __forceinline__ void three_terms(float x, float (&t)[3]) {
+    const uint32_t b = __float_as_uint(x);
+    const bool fine = (b & 0x7F800000u) != 0x7F800000u;
+    t[0] = fine ? __uint_as_float(b & 0xFFFF0000u) : x;
+    const float r = fine ? x - t[0] : 0.0f;
+    t[1] = __uint_as_float(__float_as_uint(r) & 0xFFFF0000u);
+    t[2] = r - t[1];
+}
+
+// Where the largest scaled score is this large, its rounding (2^-24 of it,
+// which s c - m in one fma leaves in the exponent: the same factor for every
+// position, but one that can leave the range) is taken off by rounding s c too.
+__device__ __forceinline__ bool far_score(float m) { return fabsf(m) > 1e6f && m > -FLT_MAX; }
+
+__device__ __forceinline__ bool word_finite(uint32_t w) {
+    return (w & 0x7F80u) != 0x7F80u && (w & 0x7F800000u) != 0x7F800000u;
+}
+__device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
+    if ((w & 0x7F80u) == 0x7F80u) w &= 0xFFFF0000u;
+    if ((w & 0x7F800000u) == 0x7F800000u) w &= 0xFFFFu;
+    return w;
+}
+
+// Byte offset of 16-byte chunk c of row j of a tile in LDS, ROW bytes a row:
+// chunks change places within their 256 bytes so that 4, 8 and 16 neighbouring
+// rows' pieces of the same columns lie on different banks.
+template <int ROW>
+__device__ __forceinline__ int lds_slot(int j, int c) {
+    static_assert(ROW == 128 || ROW == 256 || ROW == 512, "row bytes");
+    if constexpr (ROW == 128) {
+        const int line = j >> 1, f = ((line & 1) << 2) | ((line >> 1) & 3);
+        return line * 256 + (((((j & 1) << 3) | c) ^ f) << 4);
+    }
+    return j * ROW + (((c & ~15) | ((c & 15) ^ (((j & 3) << 2) | ((j >> 2) & 3)))) << 4);
+}
+// 4 rows of 16 16-bit columns, one column a lane (16 lanes; lane i's address: row i / 4, columns 4 (i % 4) ..)
+__device__ __forceinline__ v4s read_transposed(const char* p) {
+    typedef v4s __attribute__((address_space(3))) * LP;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)p);
+}
+
+lq8_status launch_few(hipStream_t s, const AttnArgs& a, PagedTypes types, int dim, int blocks, bool prefix);
+constexpr int FEW_MAX_ROWS = 32;  // packed rows launch_few takes
+lq8_status launch_tile(hipStream_t s, const AttnArgs& a, PagedTypes types, int dim, size_t tiles, bool prefix);
+constexpr int TILE_PACKED = 128;  // packed rows of a launch_tile workgroup
+
+}  // namespace lq8

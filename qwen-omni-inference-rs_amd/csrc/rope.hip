@@ -176,9 +176,9 @@ struct AppendArgs {
 };
 
 // The sequence of a row, by all threads of the workgroup; -1: none.
-__device__ __forceinline__ int sequence_of(const BatchDev& b, int row, int* first, int* count) {
+__device__ __forceinline__ int sequence_of(const BatchDev& b, int row, int* first, int* total) {
     if (!b.row_begin) {
-        *first = row, *count = 1;
+        *first = row, *total = 1;
         return row;
     }
     __shared__ int found[3];
@@ -187,10 +187,10 @@ __device__ __forceinline__ int sequence_of(const BatchDev& b, int row, int* firs
     for (int s = threadIdx.x; s < b.batch; s += RT) {
         const RowRange r = rows_of(b, s);
         // at most one sequence of an ascending row_begin has the row
-        if (row >= r.first && row - r.first < r.count) found[0] = s, found[1] = r.first, found[2] = r.count;
+        if (row >= r.first && row - r.first < r.count) found[0] = s, found[1] = r.first, found[2] = r.total;
     }
     __syncthreads();
-    *first = found[1], *count = found[2];
+    *first = found[1], *total = found[2];
     return found[0];
 }
 
@@ -223,10 +223,10 @@ __global__ __launch_bounds__(RT) void k_append(AppendArgs a) {
     constexpr int V = Vec<T>::V, UNITS = D / (2 * V);
     static_assert(RT % UNITS == 0 && 64 % UNITS == 0, "a head's threads lie in one wave");
     const int row = blockIdx.x;
-    int first, count;
-    const int seq = sequence_of(a.batch, row, &first, &count);
+    int first, total_rows;
+    const int seq = sequence_of(a.batch, row, &first, &total_rows);
     if (seq < 0) return;  // no sequence has the row
-    const int64_t slot = (int64_t)a.batch.lengths[seq] - count + (row - first);
+    const int64_t slot = (int64_t)a.batch.lengths[seq] - total_rows + (row - first);
     int page = -1;
     if (slot >= 0 && slot < (int64_t)a.batch.max_pages << a.kv.page_shift)
         page = a.batch.pages[(size_t)seq * a.batch.max_pages + (slot >> a.kv.page_shift)];
@@ -346,7 +346,7 @@ lq8_status check_pages(const lq8_kv_pages* kv, PagesDev* out) {
 
 lq8_status check_batch(const lq8_paged_batch* b, uint32_t page_size, BatchDev* out) {
     if (!b) return fail(LQ8_ERR_INVALID_ARG, "batch: null description");
-    if (b->batch > MAX_BATCH || b->rows > MAX_ROWS) return fail(LQ8_ERR_SHAPE_MISMATCH, "batch: above 65536 sequences or 2^24 rows");
+    if (b->batch > MAX_BATCH || b->rows > MAX_ROWS) return fail(LQ8_ERR_SHAPE_MISMATCH, "batch: above 65536 sequences or 2^23 rows");
     if (b->batch && b->rows) {
         if (!b->lengths || !b->pages) return fail(LQ8_ERR_INVALID_ARG, "batch: null pointer");
         if (!b->row_begin && b->rows != b->batch)
@@ -454,7 +454,7 @@ lq8_status lq8_rope_device(lq8_ctx* ctx, const lq8_rope* rope, const lq8_rope_ro
     if (!rows) return fail(LQ8_ERR_INVALID_ARG, "rope: null rows");
     if (rope->device != ctx->device) return fail(LQ8_ERR_INVALID_ARG, "rope: the handle is another device's");
     if (rows->dtype != LQ8_DTYPE_F32 && rows->dtype != LQ8_DTYPE_BF16) return fail(LQ8_ERR_DTYPE_MISMATCH, "rope: F32 or BF16 rows");
-    if (rows->rows > MAX_ROWS || rows->heads > MAX_HEADS) return fail(LQ8_ERR_SHAPE_MISMATCH, "rope: above 2^24 rows or 16384 heads");
+    if (rows->rows > MAX_ROWS || rows->heads > MAX_HEADS) return fail(LQ8_ERR_SHAPE_MISMATCH, "rope: above 2^23 rows or 16384 heads");
     if (rows->rows == 0 || rows->heads == 0) return LQ8_OK;
     const size_t es = elem_size(rows->dtype), width = (size_t)rows->heads * rope->cfg.head_dim;
     size_t xs = rows->x_stride, ys = rows->y_stride, ps = rows->positions_stride;

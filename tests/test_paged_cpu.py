@@ -65,7 +65,7 @@ REFUSED = [
     (kv(), batch(max_pages=0), rows(), None, lq8.ShapeMismatch),
     (kv(page_size=1024), batch(max_pages=2 ** 21), rows(), None, lq8.ShapeMismatch),
     (kv(), batch(batch=65537, rows=65537), rows(), None, lq8.ShapeMismatch),
-    (kv(), batch(rows=2 ** 24 + 1, row_begin=P()), rows(), None, lq8.ShapeMismatch),
+    (kv(), batch(rows=2 ** 23 + 1, row_begin=P()), rows(), None, lq8.ShapeMismatch),
     (kv(), batch(), rows(q=None), None, lq8.InvalidArgument),
     (kv(), batch(), rows(out=P(0x10004)), None, lq8.InvalidArgument),
     (kv(), batch(), rows(num_heads=12), None, lq8.ShapeMismatch),
@@ -77,8 +77,11 @@ REFUSED = [
     (kv(), batch(), rows(scale=-1.0), None, lq8.InvalidArgument),
     (kv(), batch(), rows(scale=float("nan")), None, lq8.InvalidArgument),
     (kv(), batch(), rows(scale=float("inf")), None, lq8.InvalidArgument),
+    (kv(), batch(), rows(scale=3e38), None, lq8.InvalidArgument),
     (kv(), batch(), rows(dtype=BF16), None, lq8.DTypeMismatch),  # bf16 rows over f32 pages
     (kv(), batch(), rows(dtype=0), None, lq8.DTypeMismatch),
+    (kv(), batch(batch=1, rows=2 ** 21 + 1, row_begin=P(), max_rows=5), rows(), None, lq8.ShapeMismatch),  # 2^25 rows of heads
+    (kv(num_kv_heads=512), batch(batch=32768, rows=32768), rows(num_heads=512), None, lq8.ShapeMismatch),  # 2^24 workgroups
     (kv(), batch(), rows(), prefix(groups=5), lq8.ShapeMismatch),
     (kv(), batch(), rows(), prefix(seq_begin=None), lq8.InvalidArgument),
     (kv(), batch(), rows(), prefix(max_pages=0), lq8.ShapeMismatch),
