@@ -22,8 +22,8 @@ struct RopePair {
 
 constexpr int PAGE_MIN = 16, PAGE_MAX = 1024;
 constexpr uint32_t MAX_KV_HEADS = 1024, MAX_HEADS = 16384, MAX_BATCH = 65536;
-// a launch has at most 2^32 threads: 256 of a row, 64 of a row's head
-constexpr uint32_t MAX_ROWS = 1u << 23, MAX_ROW_HEADS = 1u << 25;
+// a launch has at most 2^32 threads, and there may be 256 of a row, or of a row's head
+constexpr uint32_t MAX_ROWS = 1u << 23, MAX_ROW_HEADS = 1u << 23;
 
 // Element types of a call: rows in T, pages in C.
 enum PagedTypes : int { PT_F32_F32 = 0, PT_F32_BF16 = 1, PT_BF16_BF16 = 2 };

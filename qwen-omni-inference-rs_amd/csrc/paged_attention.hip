@@ -8,81 +8,123 @@
 namespace lq8 {
 namespace {
 
-// The row's pieces together: o = sum 2^(m_c - m) o_c / sum 2^(m_c - m) l_c, a
-// wave per (row, head), own pieces first.
-constexpr int JOIN_WAVES = 4;
-template <typename T, int D>
-__global__ __launch_bounds__(64 * JOIN_WAVES) void k_join(AttnArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int64_t item = (int64_t)blockIdx.x * JOIN_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// The row's pieces together: o = sum 2^(m_c - m) o_c / sum 2^(m_c - m) l_c.
+// head_dim / 4 lanes take four elements each of a (row, head); SUB such groups
+// share its pieces, every SUB-th each, U of them in flight, and meet in LDS.
+constexpr int JOIN_THREADS = 256;
+template <typename T, int D, int SUB>
+__global__ __launch_bounds__(JOIN_THREADS) void k_join(AttnArgs a) {
+    constexpr int LANES = D / 4, GROUPS = JOIN_THREADS / LANES, U = SUB == 1 ? 8 : 4;
+    const int tid = threadIdx.x, lane = tid % LANES, group = tid / LANES, sub = group % SUB;
+    const int64_t item = (int64_t)blockIdx.x * (GROUPS / SUB) + group / SUB;
     const int row = (int)(item / a.heads), head = (int)(item - (int64_t)row * a.heads);
-    if (row >= a.batch.rows) return;
-    // the row's sequence, and its group
-    int seq = row;
+    // the row's sequence, its prefix, and their pieces (none: own = pre = 0)
+    int seq = row < a.batch.rows ? row : -1;
+    auto any_lane = [&](bool mine) {  // the lowest lane of the group that has it, -1
+        const uint64_t b = (__ballot(mine) >> (tid & 63 & ~(LANES - 1))) & (~0ull >> (64 - LANES));
+        return b ? __ffsll((unsigned long long)b) - 1 : -1;
+    };
     if (a.batch.row_begin) {
-        seq = -1;
-        for (int s0 = 0; s0 < a.batch.batch && seq < 0; s0 += 64) {
+        int found = -1;
+        for (int s0 = 0; s0 < a.batch.batch; s0 += LANES) {
             bool mine = false;
-            if (s0 + lane < a.batch.batch) {
+            if (seq >= 0 && s0 + lane < a.batch.batch) {
                 const RowRange r = rows_of(a.batch, s0 + lane);
                 mine = row >= r.first && row - r.first < r.count;
             }
-            const uint64_t b = __ballot(mine);
-            if (b) seq = s0 + __ffsll((unsigned long long)b) - 1;
+            const int w = any_lane(mine);
+            if (w >= 0 && found < 0) found = s0 + w;
         }
-        if (seq < 0) return;  // behind the last sequence
+        seq = found;
     }
-    int group = -1;
-    for (int g0 = 0; g0 < a.prefix.groups && group < 0; g0 += 64) {
-        const bool mine = g0 + lane < a.prefix.groups && seq >= a.prefix.seq_begin[g0 + lane] && seq < a.prefix.seq_begin[g0 + lane + 1];
-        const uint64_t b = __ballot(mine);
-        if (b) group = g0 + __ffsll((unsigned long long)b) - 1;
+    int prefix = -1;
+    for (int g0 = 0; g0 < a.prefix.groups; g0 += LANES) {
+        const int w = any_lane(g0 + lane < a.prefix.groups && seq >= a.prefix.seq_begin[g0 + lane] && seq < a.prefix.seq_begin[g0 + lane + 1]);
+        if (w >= 0 && prefix < 0) prefix = g0 + w;
     }
-    const Span s = own_span(a, seq);
-    const int sees = s.sees(row - s.first), len = piece_len(s.length, a.own);
-    const int own = (sees + len - 1) / len;
-    int pre = 0;
-    if (group >= 0) {
-        const int n = held(a.prefix.lengths[group], a.prefix.max_pages, a.kv.page_shift);
-        const int plen = piece_len(n, a.pre);
-        pre = (n + plen - 1) / plen;
+    int own = 0, pre = 0;
+    if (seq >= 0) {
+        const Span s = own_span(a, seq);
+        const int len = piece_len(s.length, a.own);
+        own = (s.sees(row - s.first) + len - 1) / len;
+        if (prefix >= 0) {
+            const int n = held(a.prefix.lengths[prefix], a.prefix.max_pages, a.kv.page_shift), plen = piece_len(n, a.pre);
+            pre = (n + plen - 1) / plen;
+        }
     }
     const size_t step = (size_t)a.batch.rows * a.heads;
-    auto at = [&](int c) { return (size_t)(c < own ? c : a.own.pieces + c - own) * step + item; };
-    float m = -__builtin_huge_valf();
-    for (int c = lane; c < own + pre; c += 64) m = fmaxf(m, a.ml[at(c)].x);
-    for (int d = 32; d > 0; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
-    const bool none = m == -__builtin_huge_valf();  // no piece saw anything
-    const float mu = fmaxf(m, -FLT_MAX);
-    float l = 0.0f, o[D / 64];
+    float m = -__builtin_huge_valf(), l = 0.0f;
+    v4f o = {0, 0, 0, 0};
+    for (int c0 = sub; c0 < own + pre; c0 += SUB * U) {
+        float2 ml[U];
+        v4f y[U];
 #pragma unroll
-    for (int k = 0; k < D / 64; k++) o[k] = 0.0f;
-#pragma unroll 4
-    for (int c = 0; c < own + pre; c++) {
-        const size_t k = at(c);
-        const float2 ml = a.ml[k];
-        const float f = __builtin_amdgcn_exp2f(ml.x - mu);
-        l = fmaf(f, ml.y, l);
-        const float* y = a.part + k * D + (D / 64) * lane;
+        for (int u = 0; u < U; u++) {
+            const int c = min(c0 + u * SUB, own + pre - 1);
+            const size_t at = (size_t)(c < own ? c : a.own.pieces + c - own) * step + item;
+            ml[u] = a.ml[at];
+            y[u] = *(const v4f*)(a.part + at * D + 4 * lane);
+        }
+        float mn = m;
 #pragma unroll
-        for (int e = 0; e < D / 64; e++) o[e] = fmaf(f, y[e], o[e]);
+        for (int u = 0; u < U; u++) {
+            if (c0 + u * SUB >= own + pre) ml[u].x = -__builtin_huge_valf();
+            mn = fmaxf(mn, ml[u].x);
+        }
+        const float mu = fmaxf(mn, -FLT_MAX), f = __builtin_amdgcn_exp2f(m - mu);
+        l *= f;
+        o *= f;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (c0 + u * SUB >= own + pre) continue;
+            const float w = __builtin_amdgcn_exp2f(ml[u].x - mu);
+            l = fmaf(w, ml[u].y, l);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = fmaf(w, y[u][e], o[e]);
+        }
+        m = mn;
     }
-    const float inv = 1.0f / l;
-    T* out = (T*)a.out + (size_t)row * a.os + (size_t)head * D + (D / 64) * lane;
+    if constexpr (SUB > 1) {
+        __shared__ float2 sml[GROUPS];
+        __shared__ v4f so[GROUPS][LANES];
+        if (lane == 0) sml[group] = make_float2(m, l);
+        so[group][lane] = o;
+        __syncthreads();
+        if (sub) return;
+        float mn = m;
 #pragma unroll
-    for (int e = 0; e < D / 64; e++) {
-        const float y = none ? 0.0f : o[e] * inv;
-        if constexpr (sizeof(T) == 4) out[e] = y;
-        else out[e].bits = __builtin_bit_cast(uint16_t, (__bf16)y);
+        for (int u = 1; u < SUB; u++) mn = fmaxf(mn, sml[group + u].x);
+        const float mu = fmaxf(mn, -FLT_MAX), f = __builtin_amdgcn_exp2f(m - mu);
+        l *= f;
+        o *= f;
+#pragma unroll
+        for (int u = 1; u < SUB; u++) {
+            const float w = __builtin_amdgcn_exp2f(sml[group + u].x - mu);
+            l = fmaf(w, sml[group + u].y, l);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = fmaf(w, so[group + u][lane][e], o[e]);
+        }
+        m = mn;
     }
+    if (seq < 0) return;  // behind the last sequence
+    o = m == -__builtin_huge_valf() ? v4f{0, 0, 0, 0} : o * (1.0f / l);  // (no piece saw anything)
+    const size_t at = (size_t)row * a.os + (size_t)head * D + 4 * lane;
+    if constexpr (sizeof(T) == 4) *(v4f*)((float*)a.out + at) = o;
+    else *(uint2*)((uint16_t*)a.out + at) = make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
 }
 
-lq8_status launch_join(const AttnArgs& a, bool f32, int dim, hipStream_t s) {
-    const dim3 grid((unsigned)(((size_t)a.batch.rows * a.heads + JOIN_WAVES - 1) / JOIN_WAVES)), block(64 * JOIN_WAVES);
-    if (f32 && dim == 64) hipLaunchKernelGGL((k_join<float, 64>), grid, block, 0, s, a);
-    else if (f32) hipLaunchKernelGGL((k_join<float, 128>), grid, block, 0, s, a);
-    else if (dim == 64) hipLaunchKernelGGL((k_join<Bf16, 64>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((k_join<Bf16, 128>), grid, block, 0, s, a);
+template <typename T, int D>
+void launch_join_sub(const AttnArgs& a, size_t slots, hipStream_t s) {
+    // up to eight pieces a group takes at once; more are shared by eight groups
+    const size_t items = (size_t)a.batch.rows * a.heads, groups = JOIN_THREADS / (D / 4);
+    if (slots <= 8) hipLaunchKernelGGL((k_join<T, D, 1>), dim3((unsigned)((items + groups - 1) / groups)), dim3(JOIN_THREADS), 0, s, a);
+    else hipLaunchKernelGGL((k_join<T, D, 8>), dim3((unsigned)((items + groups / 8 - 1) / (groups / 8))), dim3(JOIN_THREADS), 0, s, a);
+}
+lq8_status launch_join(const AttnArgs& a, bool f32, int dim, size_t slots, hipStream_t s) {
+    if (f32 && dim == 64) launch_join_sub<float, 64>(a, slots, s);
+    else if (f32) launch_join_sub<float, 128>(a, slots, s);
+    else if (dim == 64) launch_join_sub<Bf16, 64>(a, slots, s);
+    else launch_join_sub<Bf16, 128>(a, slots, s);
     LQ8_HIP(hipGetLastError());
     return LQ8_OK;
 }
@@ -95,22 +137,26 @@ struct Plan {
     size_t slots = 0, scratch = 0;        // of partial results; their bytes
 };
 
+constexpr int FEW_FILL = 8, TILE_FILL = 2;
+
 // Pieces of a part whose positions are at most `most`, in `groups` workgroups
 // a piece.  few: its kernel takes spans one by one, so that a long one among
 // short ones needs pieces of its own.
 Cut cut_of(size_t most, size_t groups, int cus, bool few, bool f32_pages) {
     Cut c;
+    size_t pieces;
     if (few) {
         c.unit = f32_pages ? 64 : 128;  // a tile for each of the four waves
         c.shortest = c.unit;
-        const size_t fill = 4 * (size_t)cus / groups, longest = (most + 4095) / 4096, cap = 16384 / groups;
-        c.pieces = (int)std::max<size_t>(1, std::max(fill, std::min(longest, cap)));
+        const size_t longest = (most + 2047) / 2048, cap = 32768 / groups;
+        pieces = std::max((size_t)FEW_FILL * cus / groups, std::min(longest, cap));
     } else {
         c.unit = f32_pages ? 32 : 64;
         c.shortest = 256;
-        c.pieces = (int)std::max<size_t>(1, 2 * (size_t)cus / groups);
+        pieces = (size_t)TILE_FILL * cus / groups;
     }
-    c.pieces = (int)std::min<size_t>(c.pieces, std::max<size_t>(1, (most + c.shortest - 1) / c.shortest));
+    c.shift = __builtin_ctz(c.shortest);
+    c.pieces = (int)std::max<size_t>(1, std::min(pieces, (most + c.shortest - 1) / c.shortest));
     return c;
 }
 
@@ -156,9 +202,8 @@ lq8_status check_attention(const lq8_kv_pages* kv, const lq8_paged_batch* batch,
     if ((st = check_types(rows->dtype, kv->dtype, types))) return st;
     if (rows->num_heads == 0 || rows->num_heads > MAX_HEADS || rows->num_heads % kv->num_kv_heads)
         return fail(LQ8_ERR_SHAPE_MISMATCH, "attention: num_heads must be a multiple of num_kv_heads, up to 16384");
-    // (a launch has at most 2^32 threads, a wave of which joins a row's head)
     if ((uint64_t)batch->rows * rows->num_heads > MAX_ROW_HEADS)
-        return fail(LQ8_ERR_SHAPE_MISMATCH, "attention: rows * num_heads above 2^25");
+        return fail(LQ8_ERR_SHAPE_MISMATCH, "attention: rows * num_heads above 2^23");
     if (!(rows->scale > 0.0f) || !std::isfinite(rows->scale * 1.4426950408889634f))
         return fail(LQ8_ERR_INVALID_ARG, "attention: scale must be positive and finite");
     const size_t es = rows->dtype == LQ8_DTYPE_F32 ? 4 : 2, width = (size_t)rows->num_heads * kv->head_dim;
@@ -202,7 +247,7 @@ lq8_status attention(lq8_ctx* ctx, const lq8_kv_pages* kv, const lq8_paged_batch
     }
     st = p.own_few ? launch_few(ctx->stream, a, types, dim, p.own_blocks, false) : launch_tile(ctx->stream, a, types, dim, p.own_tiles, false);
     if (st || p.slots == 1) return st;
-    return launch_join(a, rows->dtype == LQ8_DTYPE_F32, dim, ctx->stream);
+    return launch_join(a, rows->dtype == LQ8_DTYPE_F32, dim, p.slots, ctx->stream);
 }
 
 }  // namespace

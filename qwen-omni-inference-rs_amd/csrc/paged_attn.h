@@ -28,8 +28,9 @@ struct PrefixDev {
 
 struct Cut {
     int pieces = 1;     // at most
-    int shortest = 64;  // positions of the shortest piece, a multiple of the kernel's tile
-    int unit = 64;      // pieces are multiples of it
+    int shortest = 64;  // positions of the shortest piece, a power of two
+    int shift = 6;      // its logarithm
+    int unit = 64;      // pieces are multiples of it, a power of two up to `shortest`
 };
 
 struct AttnArgs {
@@ -47,10 +48,9 @@ struct AttnArgs {
 };
 
 __host__ __device__ inline int piece_len(int length, const Cut& c) {
-    const int n0 = (length + c.shortest - 1) / c.shortest;
-    const int n = n0 < c.pieces ? (n0 < 1 ? 1 : n0) : c.pieces;
-    const int len = (length + n - 1) / n;
-    return len < 1 ? c.unit : (len + c.unit - 1) / c.unit * c.unit;
+    const int n = (int)(((unsigned)length + c.shortest - 1) >> c.shift);
+    if (n <= c.pieces) return c.shortest;
+    return (int)(((unsigned)(length + c.pieces - 1) / (unsigned)c.pieces + c.unit - 1) & ~(unsigned)(c.unit - 1));
 }
 
 // What one workgroup's rows attend to.
@@ -77,24 +77,32 @@ __device__ __forceinline__ Span prefix_span(const AttnArgs& a, int g) {
             held(a.prefix.lengths[g], a.prefix.max_pages, a.kv.page_shift), 1 << 30};
 }
 
-// The page of position j, -1 where none holds it.
+// The page of position j (the same for the whole wave), -1 where none holds
+// it.  The entry is loaded whether j exists or not (that of the last position
+// before `end` then, end > 0), by a scalar load.
+typedef const int32_t __attribute__((address_space(4))) * ScalarInts;
 __device__ __forceinline__ int page_at(const AttnArgs& a, const Span& s, int j, int end) {
-    if (j >= end) return -1;
-    const int p = s.table[j >> a.kv.page_shift];
-    return (unsigned)p < (unsigned)a.kv.num_pages ? p : -1;
+    const int at = __builtin_amdgcn_readfirstlane(min(j, end - 1) >> a.kv.page_shift);
+    const int p = ((ScalarInts)s.table)[at];
+    const bool there = (j < end) & ((unsigned)p < (unsigned)a.kv.num_pages);
+    return there ? p : -1;
 }
-// Element offset of position j (in page p) of kv head g; p < 0: of the cache's first slots, which are there to be read.
+// Element offset of position j (in page p) of kv head g; p < 0: of a slot of page 0, which is there to be read.
 __device__ __forceinline__ size_t slot_off(const AttnArgs& a, int p, int g, int j, int dim) {
-    return p < 0 ? 0 : p * a.kv.page_stride + (((size_t)g << a.kv.page_shift) + (j & ((1 << a.kv.page_shift) - 1))) * dim;
+    return max(p, 0) * a.kv.page_stride + (size_t)(unsigned)(((g << a.kv.page_shift) + (j & ((1 << a.kv.page_shift) - 1))) * dim);
 }
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef short v4s __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
+// to nearest, ties to even, NaN kept (one instruction for both)
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-    return (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (__bf16)b) << 16);
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2b));
 }
 __device__ __forceinline__ float low_bf16(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float high_bf16(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
@@ -111,19 +119,18 @@ __device__ __forceinline__ void three_terms(float x, float (&t)[3]) {
     t[2] = r - t[1];
 }
 
+__device__ __forceinline__ v8b join_halves(v4s a, v4s b) {
+    return __builtin_bit_cast(v8b, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// A loaded value waited for here: used inside a loop it would otherwise be
+// waited for there, and with it, loads returning in order, the loop's own.
+template <typename T> __device__ __forceinline__ void arrived(T& x) { asm volatile("" : "+v"(x)); }
+
 // Where the largest scaled score is this large, its rounding (2^-24 of it,
 // which s c - m in one fma leaves in the exponent: the same factor for every
 // position, but one that can leave the range) is taken off by rounding s c too.
 __device__ __forceinline__ bool far_score(float m) { return fabsf(m) > 1e6f && m > -FLT_MAX; }
-
-__device__ __forceinline__ bool word_finite(uint32_t w) {
-    return (w & 0x7F80u) != 0x7F80u && (w & 0x7F800000u) != 0x7F800000u;
-}
-__device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
-    if ((w & 0x7F80u) == 0x7F80u) w &= 0xFFFF0000u;
-    if ((w & 0x7F800000u) == 0x7F800000u) w &= 0xFFFFu;
-    return w;
-}
 
 // Byte offset of 16-byte chunk c of row j of a tile in LDS, ROW bytes a row:
 // chunks change places within their 256 bytes so that 4, 8 and 16 neighbouring
@@ -141,6 +148,26 @@ __device__ __forceinline__ int lds_slot(int j, int c) {
 __device__ __forceinline__ v4s read_transposed(const char* p) {
     typedef v4s __attribute__((address_space(3))) * LP;
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)p);
+}
+
+// Sets a sign bit of `bits` where w, two bf16 or a float32, is not finite: an
+// exponent of ones carries into it.
+template <bool F32>
+__device__ __forceinline__ void mark_odd(v4u v, uint32_t& bits) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) bits |= F32 ? (v[e] & 0x7FFFFFFFu) + 0x00800000u : (v[e] & 0x7FFF7FFFu) + 0x00800080u;
+}
+template <bool F32>
+__device__ __forceinline__ bool is_odd(uint32_t bits) { return (bits & (F32 ? 0x80000000u : 0x80008000u)) != 0; }
+// v with zeros in place of what is not finite
+template <bool F32>
+__device__ __forceinline__ v4u finite_part(v4u v) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if ((v[e] & 0x7F800000u) == 0x7F800000u) v[e] &= F32 ? 0u : 0xFFFFu;
+        if (!F32 && (v[e] & 0x7F80u) == 0x7F80u) v[e] &= 0xFFFF0000u;
+    }
+    return v;
 }
 
 lq8_status launch_few(hipStream_t s, const AttnArgs& a, PagedTypes types, int dim, int blocks, bool prefix);

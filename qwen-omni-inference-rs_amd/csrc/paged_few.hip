@@ -33,20 +33,20 @@ template <int D> struct TileB {
     static constexpr int KS = D / 32;       // products of a score block
     static constexpr int VI = D / 16;       // 16-byte loads of V per lane
     static constexpr int RPI = 512 / D;     // rows a wave's load covers
-    uint4 k[2][KS], v[VI];
+    v4u k[2][KS], v[VI];
 };
 template <int D> struct TileF {
     static constexpr int N = 16;
     static constexpr int KS = D / 16;       // 16-byte loads of K per lane
     static constexpr int VH = D / 64;
-    float4 k[KS], v[4][VH];
+    v4f k[KS], v[4][VH];
 };
 template <int D> struct Tile<PT_BF16_BF16, D> : TileB<D> {};
 template <int D> struct Tile<PT_F32_BF16, D> : TileB<D> {};
 template <int D> struct Tile<PT_F32_F32, D> : TileF<D> {};
 
 template <int TYPES, int D, int MB, bool PREFIX>
-__global__ __launch_bounds__(64 * WAVES) void k_few(AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, MB == 1 ? 2 : 1) void k_few(AttnArgs a) {
     constexpr bool F32C = TYPES == PT_F32_F32, F32Q = TYPES != PT_BF16_BF16;
     constexpr int TERMS = TYPES == PT_F32_BF16 ? 3 : 1;
     typedef Tile<TYPES, D> T;
@@ -100,9 +100,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_few(AttnArgs a) {
             const float* qp = (const float*)a.q + row * a.qs + (size_t)head * D + 8 * p;
 #pragma unroll
             for (int t = 0; t < D / 32; t++) {
-                float y[8];
-                *(float4*)y = *(const float4*)(qp + 32 * t);
-                *(float4*)(y + 4) = *(const float4*)(qp + 32 * t + 4);
+                const float4 y0 = *(const float4*)(qp + 32 * t), y1 = *(const float4*)(qp + 32 * t + 4);
+                const float y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     float t0[3], t1[3];
@@ -116,8 +115,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_few(AttnArgs a) {
             const uint16_t* qp = (const uint16_t*)a.q + row * a.qs + (size_t)head * D + 8 * p;
 #pragma unroll
             for (int t = 0; t < D / 32; t++) {
-                const uint4 v = *(const uint4*)(qp + 32 * t);
-                q[mb][0][t][0] = v.x, q[mb][0][t][1] = v.y, q[mb][0][t][2] = v.z, q[mb][0][t][3] = v.w;
+                const v4u v = *(const v4u*)(qp + 32 * t);
+                q[mb][0][t][0] = v[0], q[mb][0][t][1] = v[1], q[mb][0][t][2] = v[2], q[mb][0][t][3] = v[3];
             }
         }
     }
@@ -138,13 +137,13 @@ __global__ __launch_bounds__(64 * WAVES) void k_few(AttnArgs a) {
         if constexpr (F32C) {
             const float* kp = (const float*)kc + off[0] + r * D + 4 * p;
 #pragma unroll
-            for (int t = 0; t < T::KS; t++) tile.k[t] = *(const float4*)(kp + 16 * t);
+            for (int t = 0; t < T::KS; t++) tile.k[t] = *(const v4f*)(kp + 16 * t);
         } else {
 #pragma unroll
             for (int b = 0; b < BLOCKS; b++) {
                 const uint16_t* kp = (const uint16_t*)kc + off[b] + r * D + 8 * p;
 #pragma unroll
-                for (int t = 0; t < T::KS; t++) tile.k[b][t] = *(const uint4*)(kp + 32 * t);
+                for (int t = 0; t < T::KS; t++) tile.k[b][t] = *(const v4u*)(kp + 32 * t);
             }
         }
     };
@@ -154,12 +153,12 @@ __global__ __launch_bounds__(64 * WAVES) void k_few(AttnArgs a) {
 #pragma unroll
             for (int v = 0; v < 4; v++)
 #pragma unroll
-                for (int h = 0; h < T::VH; h++) tile.v[v][h] = *(const float4*)(vp + v * D + 64 * h);
+                for (int h = 0; h < T::VH; h++) tile.v[v][h] = *(const v4f*)(vp + v * D + 64 * h);
         } else {
 #pragma unroll
             for (int i = 0; i < T::VI; i++) {
                 const uint16_t* vp = (const uint16_t*)vc + off[i * T::RPI / 16] + (i * T::RPI % 16) * D + lane * 8;
-                tile.v[i] = *(const uint4*)vp;
+                tile.v[i] = *(const v4u*)vp;
             }
         }
     };
@@ -175,10 +174,24 @@ __global__ __launch_bounds__(64 * WAVES) void k_few(AttnArgs a) {
     int pg[BLOCKS], pn[BLOCKS];
     size_t off[BLOCKS], on[BLOCKS];
     int j = beg + N * w;
-    pages_of(j, pg, off);
     if (j < end) {
+        pages_of(j, pg, off);
         load_k(off);
         load_v(off);
+    }
+#pragma unroll
+    for (int mb = 0; mb < MB; mb++) {
+        if constexpr (F32C) {
+#pragma unroll
+            for (int t = 0; t < D / 4; t++) arrived(qf[mb][t]);
+        } else {
+#pragma unroll
+            for (int z = 0; z < TERMS; z++)
+#pragma unroll
+                for (int t = 0; t < D / 32; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) arrived(q[mb][z][t][e]);
+        }
     }
     for (; j < end; j += N * WAVES) {
         const int jn = j + N * WAVES;
@@ -193,17 +206,17 @@ __global__ __launch_bounds__(64 * WAVES) void k_few(AttnArgs a) {
                 if constexpr (F32C) {
 #pragma unroll
                     for (int i = 0; i < T::KS; i++) {
-                        t = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.k[i].x, qf[mb][4 * i], t, 0, 0, 0);
-                        t = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.k[i].y, qf[mb][4 * i + 1], t, 0, 0, 0);
-                        t = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.k[i].z, qf[mb][4 * i + 2], t, 0, 0, 0);
-                        t = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.k[i].w, qf[mb][4 * i + 3], t, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.k[i][0], qf[mb][4 * i], t, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.k[i][1], qf[mb][4 * i + 1], t, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.k[i][2], qf[mb][4 * i + 2], t, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.k[i][3], qf[mb][4 * i + 3], t, 0, 0, 0);
                     }
                 } else {
 #pragma unroll
                     for (int z = TERMS - 1; z >= 0; z--)
 #pragma unroll
                         for (int i = 0; i < T::KS; i++) {
-                            const uint4 qv = make_uint4(q[mb][z][i][0], q[mb][z][i][1], q[mb][z][i][2], q[mb][z][i][3]);
+                            const v4u qv = v4u{q[mb][z][i][0], q[mb][z][i][1], q[mb][z][i][2], q[mb][z][i][3]};
                             t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, tile.k[b][i]),
                                                                        __builtin_bit_cast(v8b, qv), t, 0, 0, 0);
                         }
@@ -285,22 +298,24 @@ __global__ __launch_bounds__(64 * WAVES) void k_few(AttnArgs a) {
         bool odd = false;
         if constexpr (F32C) {
             if (masked) {
+                uint32_t bits = 0;
 #pragma unroll
                 for (int v = 0; v < 4; v++) {
                     const bool gone = hole || j + 4 * p + v >= end;
 #pragma unroll
                     for (int h = 0; h < T::VH; h++) {
-                        float* y = (float*)&tile.v[v][h];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            if (gone) y[e] = 0.0f;
-                            const bool bad = !(fabsf(y[e]) < __builtin_huge_valf());
-                            odd |= bad;
-                            if (bad) y[e] = 0.0f;
-                        }
+                        if (gone) tile.v[v][h] = v4f{0, 0, 0, 0};
+                        mark_odd<true>(__builtin_bit_cast(v4u, tile.v[v][h]), bits);
                     }
                 }
-                odd = __any(odd);
+                odd = __any(is_odd<true>(bits));
+                if (odd) {
+#pragma unroll
+                    for (int v = 0; v < 4; v++)
+#pragma unroll
+                        for (int h = 0; h < T::VH; h++)
+                            tile.v[v][h] = __builtin_bit_cast(v4f, finite_part<true>(__builtin_bit_cast(v4u, tile.v[v][h])));
+                }
             }
 #pragma unroll
             for (int mb = 0; mb < MB; mb++)
@@ -309,38 +324,33 @@ __global__ __launch_bounds__(64 * WAVES) void k_few(AttnArgs a) {
 #pragma unroll
                     for (int h = 0; h < T::VH; h++) {
                         const float y = sc[mb][0][v];
-                        acc[mb][4 * h] = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.v[v][h].x, y, acc[mb][4 * h], 0, 0, 0);
-                        acc[mb][4 * h + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.v[v][h].y, y, acc[mb][4 * h + 1], 0, 0, 0);
-                        acc[mb][4 * h + 2] = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.v[v][h].z, y, acc[mb][4 * h + 2], 0, 0, 0);
-                        acc[mb][4 * h + 3] = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.v[v][h].w, y, acc[mb][4 * h + 3], 0, 0, 0);
+                        acc[mb][4 * h] = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.v[v][h][0], y, acc[mb][4 * h], 0, 0, 0);
+                        acc[mb][4 * h + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.v[v][h][1], y, acc[mb][4 * h + 1], 0, 0, 0);
+                        acc[mb][4 * h + 2] = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.v[v][h][2], y, acc[mb][4 * h + 2], 0, 0, 0);
+                        acc[mb][4 * h + 3] = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.v[v][h][3], y, acc[mb][4 * h + 3], 0, 0, 0);
                     }
             if (jn < end) load_v(on);
         } else {
-            if (masked || TERMS > 1) {
+            if (masked) {
 #pragma unroll
                 for (int i = 0; i < T::VI; i++) {
                     const int row = i * T::RPI + lane / (D / 8);
-                    const bool gone = masked && (pg[i * T::RPI / 16] < 0 || j + row >= end);
-                    uint32_t* y = (uint32_t*)&tile.v[i];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        if (gone) y[e] = 0;
-                        odd |= !word_finite(y[e]);
-                    }
+                    if (pg[i * T::RPI / 16] < 0 || j + row >= end) tile.v[i] = v4u{0, 0, 0, 0};
                 }
-                odd = __any(odd);
+            }
+            if (masked || TERMS > 1) {
+                uint32_t bits = 0;
+#pragma unroll
+                for (int i = 0; i < T::VI; i++) mark_odd<false>(tile.v[i], bits);
+                odd = __any(is_odd<false>(bits));
                 if (odd) {
 #pragma unroll
-                    for (int i = 0; i < T::VI; i++) {
-                        uint32_t* y = (uint32_t*)&tile.v[i];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) y[e] = finite_halves(y[e]);
-                    }
+                    for (int i = 0; i < T::VI; i++) tile.v[i] = finite_part<false>(tile.v[i]);
                 }
             }
 #pragma unroll
             for (int i = 0; i < T::VI; i++)
-                *(uint4*)(own + lds_slot<2 * D>(i * T::RPI + lane / (D / 8), lane % (D / 8))) = tile.v[i];
+                *(v4u*)(own + lds_slot<2 * D>(i * T::RPI + lane / (D / 8), lane % (D / 8))) = tile.v[i];
             if (jn < end) load_v(on);
             __builtin_amdgcn_wave_barrier();
             uint32_t pb[MB][TERMS][4];
@@ -364,17 +374,14 @@ __global__ __launch_bounds__(64 * WAVES) void k_few(AttnArgs a) {
             // lane -> (row 4 p + r / 4 of each block, 4 of 16 columns)
 #pragma unroll
             for (int t = 0; t < DT; t++) {
-                v4s lo, hi;
                 const int row = 4 * p + (r >> 2), ch = 2 * t + ((r >> 1) & 1), in = 8 * (r & 1);
-                lo = read_transposed(own + lds_slot<2 * D>(row, ch) + in);
-                hi = read_transposed(own + lds_slot<2 * D>(row + 16, ch) + in);
-                struct { v4s x, y; } both = {lo, hi};
-                const v8b va = __builtin_bit_cast(v8b, both);
+                const v8b va = join_halves(read_transposed(own + lds_slot<2 * D>(row, ch) + in),
+                                           read_transposed(own + lds_slot<2 * D>(row + 16, ch) + in));
 #pragma unroll
                 for (int mb = 0; mb < MB; mb++)
 #pragma unroll
                     for (int z = TERMS - 1; z >= 0; z--) {
-                        const uint4 pv = make_uint4(pb[mb][z][0], pb[mb][z][1], pb[mb][z][2], pb[mb][z][3]);
+                        const v4u pv = v4u{pb[mb][z][0], pb[mb][z][1], pb[mb][z][2], pb[mb][z][3]};
                         acc[mb][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, __builtin_bit_cast(v8b, pv), acc[mb][t], 0, 0, 0);
                     }
             }

@@ -112,9 +112,8 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
         const float* qp = (const float*)a.q + qat + 8 * p;
 #pragma unroll
         for (int t = 0; t < D / 16; t++) {
-            float y[8];
-            *(float4*)y = *(const float4*)(qp + 16 * t);
-            *(float4*)(y + 4) = *(const float4*)(qp + 16 * t + 4);
+            const float4 y0 = *(const float4*)(qp + 16 * t), y1 = *(const float4*)(qp + 16 * t + 4);
+            const float y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 float t0[3], t1[3];
@@ -128,8 +127,8 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
         const uint16_t* qp = (const uint16_t*)a.q + qat + 8 * p;
 #pragma unroll
         for (int t = 0; t < D / 16; t++) {
-            const uint4 v = *(const uint4*)(qp + 16 * t);
-            q[0][t][0] = v.x, q[0][t][1] = v.y, q[0][t][2] = v.z, q[0][t][3] = v.w;
+            const v4u v = *(const v4u*)(qp + 16 * t);
+            q[0][t][0] = v[0], q[0][t][1] = v[1], q[0][t][2] = v[2], q[0][t][3] = v[3];
         }
     }
 
@@ -141,28 +140,27 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
     float m = -__builtin_huge_valf(), l = 0.0f;
 
     // staging: chunk tid + 256 n of the tile; a wave's rows lie in one block
-    uint4 kr[CI], vr[CI];
-    int pg[BLOCKS], pn[BLOCKS];
-    size_t off[BLOCKS], on[BLOCKS];
+    v4u kr[CI], vr[CI];
+    int pg[BLOCKS], pn[BLOCKS];  // of this tile and the next
     const char *kc = (const char*)a.kv.k, *vc = (const char*)a.kv.v;
-    auto pages_of = [&](int j, int (&pg)[BLOCKS], size_t (&off)[BLOCKS]) {
+    auto pages_of = [&](int j, int (&pg)[BLOCKS]) {
 #pragma unroll
-        for (int b = 0; b < BLOCKS; b++) {
-            pg[b] = page_at(a, s, j + 16 * b, end);
-            off[b] = slot_off(a, pg[b], g, j + 16 * b, D);
-        }
+        for (int b = 0; b < BLOCKS; b++) pg[b] = page_at(a, s, j + 16 * b, end);
     };
-    auto block_of = [&](int n) { return (n * (THREADS / CPR) + w * (64 / CPR)) / 16; };
-    auto load = [&](const size_t (&off)[BLOCKS]) {
+    constexpr int RPN = THREADS / CPR;  // rows of a step
+    auto page_of = [&](const int (&pg)[BLOCKS], int n) {  // of the wave's rows of step n
+        if constexpr (RPN <= 16) return pg[n * RPN / 16];
+        else return w >= 2 ? pg[2 * n + 1] : pg[2 * n];
+    };
+    const int lane_at = (tid / CPR & 15) * ROW + tid % CPR * 16;
+    auto load = [&](const int (&pg)[BLOCKS], int j) {
 #pragma unroll
         for (int n = 0; n < CI; n++) {
-            const int row = n * (THREADS / CPR) + tid / CPR, b = block_of(n);
-            size_t o = off[0];
-#pragma unroll
-            for (int k = 1; k < BLOCKS; k++) o = b == k ? off[k] : o;
-            const size_t at = o * ES + (row & 15) * ROW + tid % CPR * 16;
-            kr[n] = *(const uint4*)(kc + at);
-            vr[n] = *(const uint4*)(vc + at);
+            const int b = RPN <= 16 ? n * RPN / 16 : 2 * n + w / 2;
+            const size_t at = slot_off(a, page_of(pg, n), g, j + 16 * b, D) * ES;
+            const int o = lane_at + (RPN < 16 ? n * RPN % 16 * ROW : 0);
+            kr[n] = *(const v4u*)(kc + at + o);
+            vr[n] = *(const v4u*)(vc + at + o);
         }
     };
     // registers -> buffer `buf`, tile number k at position j.  Values of rows
@@ -174,51 +172,62 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
 #pragma unroll
         for (int b = 0; b < BLOCKS; b++) hole |= pg[b] < 0;
         const bool check = TERMS > 1 || hole || j + N > least;
-        bool odd = false;
+        if (check) {
+            uint32_t bits = 0;
+#pragma unroll
+            for (int n = 0; n < CI; n++) {
+                if (page_of(pg, n) < 0 || j + n * RPN + tid / CPR >= end) vr[n] = v4u{0, 0, 0, 0};
+                mark_odd<F32C>(vr[n], bits);
+            }
+            if (is_odd<F32C>(bits)) {
+                odd_tile[buf] = k;
+#pragma unroll
+                for (int n = 0; n < CI; n++) vr[n] = finite_part<F32C>(vr[n]);
+            }
+        }
 #pragma unroll
         for (int n = 0; n < CI; n++) {
-            const int row = n * (THREADS / CPR) + tid / CPR, c = tid % CPR;
-            *(uint4*)(sk[buf] + lds_slot<ROW>(row, c)) = kr[n];
-            if (check) {
-                int page = pg[0];
-#pragma unroll
-                for (int b = 1; b < BLOCKS; b++) page = block_of(n) == b ? pg[b] : page;
-                const bool gone = page < 0 || j + row >= end;
-                uint32_t* y = (uint32_t*)&vr[n];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    y[e] = gone ? 0u : y[e];
-                    if constexpr (F32C) {
-                        if ((y[e] & 0x7F800000u) == 0x7F800000u) y[e] = 0u, odd = true;
-                    } else {
-                        odd |= !word_finite(y[e]);
-                        y[e] = finite_halves(y[e]);
-                    }
-                }
-            }
-            *(uint4*)(sv[buf] + lds_slot<ROW>(row, c)) = vr[n];
+            const int at = lds_slot<ROW>(n * RPN + tid / CPR, tid % CPR);
+            *(v4u*)(sk[buf] + at) = kr[n];
+            *(v4u*)(sv[buf] + at) = vr[n];
         }
-        if (odd) odd_tile[buf] = k;
     };
 
     int j = beg;
-    pages_of(j, pg, off);
-    pages_of(j + N, pn, on);
     if (j < end) {
-        load(off);
+        pages_of(j, pg);
+        pages_of(j + N, pn);
+        load(pg, j);
         __syncthreads();  // odd_tile is set up
         store(0, 0, j, pg);
+    }
+    if constexpr (F32C) {
+#pragma unroll
+        for (int t = 0; t < D / 2; t++) arrived(qf[t]);
+    } else {
+#pragma unroll
+        for (int z = 0; z < TERMS; z++)
+#pragma unroll
+            for (int t = 0; t < D / 16; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) arrived(q[z][t][e]);
     }
     for (int k = 0; j < end; k++, j += N) {
         const int buf = k & 1, jn = j + N;
         __syncthreads();
-        if (jn < end) load(on);
+        if (jn < end) load(pn, jn);
         int pnn[BLOCKS];  // a tile ahead of its loads
-        size_t onn[BLOCKS];
-        pages_of(jn + N, pnn, onn);
+        pages_of(jn + N, pnn);
         if (j < wmost) {
             const char *K = sk[buf], *V = sv[buf];
             v16f sc[SB];
+            v8b ko[F32C ? 1 : SB][F32C ? 1 : D / 16];
+            if constexpr (!F32C) {
+#pragma unroll
+                for (int b = 0; b < SB; b++)
+#pragma unroll
+                    for (int c = 0; c < D / 16; c++) ko[b][c] = *(const v8b*)(K + lds_slot<ROW>(32 * b + r, 2 * c + p));
+            }
 #pragma unroll
             for (int b = 0; b < SB; b++) {
                 v16f t;
@@ -234,11 +243,10 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
                 } else {
 #pragma unroll
                     for (int c = 0; c < D / 16; c++) {
-                        const v8b kv = *(const v8b*)(K + lds_slot<ROW>(32 * b + r, 2 * c + p));
 #pragma unroll
                         for (int z = TERMS - 1; z >= 0; z--) {
-                            const uint4 qv = make_uint4(q[z][c][0], q[z][c][1], q[z][c][2], q[z][c][3]);
-                            t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kv, __builtin_bit_cast(v8b, qv), t, 0, 0, 0);
+                            const v4u qv = v4u{q[z][c][0], q[z][c][1], q[z][c][2], q[z][c][3]};
+                            t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ko[b][c], __builtin_bit_cast(v8b, qv), t, 0, 0, 0);
                         }
                     }
                 }
@@ -270,7 +278,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
                         for (int e = 0; e < 16; e++)
                             if (sc[b][e] != sc[b][e]) {
                                 const float* qp = (const float*)a.q + qat;
-                                const uint16_t* kp = (const uint16_t*)kc + off[2 * b + e / 8] + (8 * (e / 4 % 2) + 4 * p + e % 4) * D;
+                                const uint16_t* kp = (const uint16_t*)kc + slot_off(a, pg[2 * b + e / 8], g, j + 32 * b + 16 * (e / 8), D) + (8 * (e / 4 % 2) + 4 * p + e % 4) * D;
                                 float t = 0.0f;
                                 for (int d = 0; d < D; d++) t = fmaf(qp[d], __uint_as_float((uint32_t)kp[d] << 16), t);
                                 sc[b][e] = t;
@@ -327,9 +335,13 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     const int vrow = 8 * (e / 4) + 4 * p + e % 4;
-                    float v[VW];
-                    if constexpr (VW == 4) *(v4f*)v = *(const v4f*)(V + lds_slot<ROW>(vrow, r));
-                    else *(float2*)v = *(const float2*)(V + lds_slot<ROW>(vrow, r >> 1) + 8 * (r & 1));
+                    v4f v;
+                    if constexpr (VW == 4) {
+                        v = *(const v4f*)(V + lds_slot<ROW>(vrow, r));
+                    } else {
+                        const float2 two = *(const float2*)(V + lds_slot<ROW>(vrow, r >> 1) + 8 * (r & 1));
+                        v = v4f{two.x, two.y, 0.0f, 0.0f};
+                    }
 #pragma unroll
                     for (int t = 0; t < DT; t++) acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[t], sc[0][e], acc[t], 0, 0, 0);
                 }
@@ -354,12 +366,11 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
                     const int vrow = 16 * ks + 4 * p + (i16 >> 2), ch = 2 * dh + ((i16 >> 1) & 1), in = 8 * (i16 & 1);
 #pragma unroll
                     for (int t = 0; t < DT; t++) {
-                        struct { v4s x, y; } both = {read_transposed(V + lds_slot<ROW>(vrow, ch + 4 * t) + in),
-                                                     read_transposed(V + lds_slot<ROW>(vrow + 8, ch + 4 * t) + in)};
-                        const v8b va = __builtin_bit_cast(v8b, both);
+                        const v8b va = join_halves(read_transposed(V + lds_slot<ROW>(vrow, ch + 4 * t) + in),
+                                                   read_transposed(V + lds_slot<ROW>(vrow + 8, ch + 4 * t) + in));
 #pragma unroll
                         for (int z = TERMS - 1; z >= 0; z--) {
-                            const uint4 pv = make_uint4(pb[z][0], pb[z][1], pb[z][2], pb[z][3]);
+                            const v4u pv = v4u{pb[z][0], pb[z][1], pb[z][2], pb[z][3]};
                             acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, __builtin_bit_cast(v8b, pv), acc[t], 0, 0, 0);
                         }
                     }
@@ -373,6 +384,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
 #pragma unroll
                     for (int e = 0; e < 8; e++) ps[(8 * (e / 4) + 4 * p + e % 4) * 32 + r] = sc[b / 2][8 * (b % 2) + e];
                     __builtin_amdgcn_wave_barrier();
+                    const size_t from = slot_off(a, pg[b], g, j + 16 * b, D);
                     for (int jj = 0; jj < 16 && pg[b] >= 0 && j + 16 * b + jj < end; jj++) {
                         const float y = ps[jj * 32 + r];
                         const bool see = j + 16 * b + jj < sees;
@@ -382,8 +394,8 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
                             for (int e = 0; e < 16; e++) {
                                 const int mrow = 8 * (e / 4) + 4 * p + e % 4;
                                 float v;
-                                if constexpr (F32C) v = ((const float*)vc)[off[b] + jj * D + VW * mrow + t];
-                                else v = __uint_as_float((uint32_t)((const uint16_t*)vc)[off[b] + jj * D + 32 * t + mrow] << 16);
+                                if constexpr (F32C) v = ((const float*)vc)[from + jj * D + VW * mrow + t];
+                                else v = __uint_as_float((uint32_t)((const uint16_t*)vc)[from + jj * D + 32 * t + mrow] << 16);
                                 if (!(fabsf(v) < __builtin_huge_valf()) && see) acc[t][e] = fmaf(y, v, acc[t][e]);
                             }
                     }
@@ -393,7 +405,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
         }
         if (jn < end) store(buf ^ 1, k + 1, jn, pn);
 #pragma unroll
-        for (int b = 0; b < BLOCKS; b++) pg[b] = pn[b], off[b] = on[b], pn[b] = pnn[b], on[b] = onn[b];
+        for (int b = 0; b < BLOCKS; b++) pg[b] = pn[b], pn[b] = pnn[b];
     }
 
     l += lane_xor<32>(l);

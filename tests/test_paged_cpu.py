@@ -80,8 +80,8 @@ REFUSED = [
     (kv(), batch(), rows(scale=3e38), None, lq8.InvalidArgument),
     (kv(), batch(), rows(dtype=BF16), None, lq8.DTypeMismatch),  # bf16 rows over f32 pages
     (kv(), batch(), rows(dtype=0), None, lq8.DTypeMismatch),
-    (kv(), batch(batch=1, rows=2 ** 21 + 1, row_begin=P(), max_rows=5), rows(), None, lq8.ShapeMismatch),  # 2^25 rows of heads
-    (kv(num_kv_heads=512), batch(batch=32768, rows=32768), rows(num_heads=512), None, lq8.ShapeMismatch),  # 2^24 workgroups
+    (kv(), batch(batch=1, rows=2 ** 19 + 1, row_begin=P(), max_rows=5), rows(), None, lq8.ShapeMismatch),  # 2^23 rows of heads
+    (kv(num_kv_heads=1024), batch(batch=65536, rows=8000, row_begin=P()), rows(num_heads=1024), None, lq8.ShapeMismatch),  # 2^24 workgroups
     (kv(), batch(), rows(), prefix(groups=5), lq8.ShapeMismatch),
     (kv(), batch(), rows(), prefix(seq_begin=None), lq8.InvalidArgument),
     (kv(), batch(), rows(), prefix(max_pages=0), lq8.ShapeMismatch),
