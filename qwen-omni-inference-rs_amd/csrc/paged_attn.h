@@ -170,6 +170,34 @@ __device__ __forceinline__ v4u finite_part(v4u v) {
     return v;
 }
 
+// Values that are not finite enter the products as zeros (a zero probability
+// times one of them would be NaN in rows that do not see it) and meet the rows
+// that see them here, after the sums are done: for positions from .. to - 1 in
+// runs of `run` every `step`, each(values of the position, whether the lane's
+// row sees it, its probability).  The lane's row has its query at q, sees
+// positions before `sees` and has reference m.
+template <typename T, typename C, int D, typename F>
+__device__ __forceinline__ void meet_odd(const AttnArgs& a, const Span& s, int g, int from, int to, int run, int step, int end,
+                                         const T* q, int sees, float m, F each) {
+    auto value = [](const auto* p) {
+        if constexpr (sizeof(*p) == 4) return (float)*(const float*)p;
+        else return __uint_as_float((uint32_t) * (const uint16_t*)p << 16);
+    };
+    for (int j0 = from; j0 < to; j0 += step)
+        for (int j = j0; j < min(j0 + run, end); j++) {
+            const int page = page_at(a, s, j, end);
+            if (page < 0) continue;
+            const size_t off = slot_off(a, page, g, j, D);
+            each((const C*)a.kv.v + off, j < sees, value, [&]() {
+                const C* k = (const C*)a.kv.k + off;
+                float x = 0.0f;
+                for (int d = 0; d < D; d++) x = fmaf(value(q + d), value(k + d), x);
+                const float mu = fmaxf(m, -FLT_MAX);
+                return __builtin_amdgcn_exp2f(far_score(mu) ? x * a.c - mu : fmaf(x, a.c, -mu));
+            });
+        }
+}
+
 lq8_status launch_few(hipStream_t s, const AttnArgs& a, PagedTypes types, int dim, int blocks, bool prefix);
 constexpr int FEW_MAX_ROWS = 32;  // packed rows launch_few takes
 lq8_status launch_tile(hipStream_t s, const AttnArgs& a, PagedTypes types, int dim, size_t tiles, bool prefix);

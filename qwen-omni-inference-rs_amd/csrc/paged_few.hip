@@ -19,6 +19,8 @@
 //               products per 16-byte load with d in the order 4 r + component
 // f32 rows over bf16 pages: q and p as three bf16 terms each (three_terms),
 // every product exact, sums in float32.
+#include <type_traits>
+
 #include "paged_attn.h"
 
 namespace lq8 {
@@ -45,15 +47,21 @@ template <int D> struct Tile<PT_BF16_BF16, D> : TileB<D> {};
 template <int D> struct Tile<PT_F32_BF16, D> : TileB<D> {};
 template <int D> struct Tile<PT_F32_F32, D> : TileF<D> {};
 
+// The head dimension of element e of O's tile t in a lane of group p.
+template <bool F32C>
+__device__ __forceinline__ int column(int t, int p, int e) {
+    return F32C ? 64 * (t / 4) + 16 * p + 4 * e + t % 4 : 16 * t + 4 * p + e;
+}
+
 template <int TYPES, int D, int MB, bool PREFIX>
 __global__ __launch_bounds__(64 * WAVES, MB == 1 ? 2 : 1) void k_few(AttnArgs a) {
     constexpr bool F32C = TYPES == PT_F32_F32, F32Q = TYPES != PT_BF16_BF16;
     constexpr int TERMS = TYPES == PT_F32_BF16 ? 3 : 1;
     typedef Tile<TYPES, D> T;
     constexpr int N = T::N, M = 16 * MB, DT = D / 16;
-    // a wave's V tile; its 16 x D sums at the end; the probabilities of a fix
+    // a wave's V tile, and its 16 x D sums at the end
     constexpr int WBYTES = 16 * D * 4;
-    static_assert(WBYTES >= 32 * D * 2 && WBYTES >= N * 16 * 4, "one wave's region");
+    static_assert(WBYTES >= 32 * D * 2, "one wave's region");
     __shared__ __attribute__((aligned(16))) char sm[WAVES * WBYTES];
     __shared__ float2 sml[WAVES][M];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, p = lane >> 4;
@@ -173,7 +181,7 @@ __global__ __launch_bounds__(64 * WAVES, MB == 1 ? 2 : 1) void k_few(AttnArgs a)
 
     int pg[BLOCKS], pn[BLOCKS];
     size_t off[BLOCKS], on[BLOCKS];
-    int j = beg + N * w;
+    int j = beg + N * w, odd_lo = INT32_MAX, odd_hi = 0;  // odd: the wave's tiles with values that are not finite
     if (j < end) {
         pages_of(j, pg, off);
         load_k(off);
@@ -294,7 +302,7 @@ __global__ __launch_bounds__(64 * WAVES, MB == 1 ? 2 : 1) void k_few(AttnArgs a)
                 }
         }
         // values: rows no row sees are zeroed, and so is what is not finite
-        // where some row must not meet it (added to the others below)
+        // where some row must not meet it (meet_odd)
         bool odd = false;
         if constexpr (F32C) {
             if (masked) {
@@ -387,37 +395,34 @@ __global__ __launch_bounds__(64 * WAVES, MB == 1 ? 2 : 1) void k_few(AttnArgs a)
             }
             __builtin_amdgcn_wave_barrier();
         }
-        if (odd) {
-            // the values that are not finite, for the rows that see them
-            float* ps = (float*)own;  // [N][16]
-#pragma unroll
-            for (int mb = 0; mb < MB; mb++) {
-#pragma unroll
-                for (int b = 0; b < BLOCKS; b++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) ps[(16 * b + 4 * p + e) * 16 + r] = sc[mb][b][e];
-                __builtin_amdgcn_wave_barrier();
-                for (int jj = 0; jj < N && j + jj < end; jj++) {
-                    int page = pg[0];
-                    size_t from = off[0];
-                    if (BLOCKS > 1 && jj >= 16) page = pg[BLOCKS - 1], from = off[BLOCKS - 1];
-                    if (page < 0) continue;
-                    const float y = ps[jj * 16 + r];
-#pragma unroll
-                    for (int t = 0; t < DT; t++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            float v;
-                            if constexpr (F32C) v = ((const float*)vc)[from + (jj & 15) * D + 64 * (t / 4) + 16 * p + 4 * e + t % 4];
-                            else v = __uint_as_float((uint32_t)((const uint16_t*)vc)[from + (jj & 15) * D + 16 * t + 4 * p + e] << 16);
-                            if (!(fabsf(v) < __builtin_huge_valf()) && j + jj < sees[mb]) acc[mb][t][e] = fmaf(y, v, acc[mb][t][e]);
-                        }
-                }
-                __builtin_amdgcn_wave_barrier();
-            }
-        }
+        if (odd) odd_lo = min(odd_lo, j), odd_hi = j + N;
 #pragma unroll
         for (int b = 0; b < BLOCKS; b++) pg[b] = pn[b], off[b] = on[b];
+    }
+
+    if (odd_hi) {
+        typedef typename std::conditional<F32Q, float, uint16_t>::type TQ;
+        typedef typename std::conditional<F32C, float, uint16_t>::type TC;
+#pragma unroll
+        for (int mb = 0; mb < MB; mb++) {
+            const TQ* qp = (const TQ*)a.q + (at[mb] / a.heads) * a.qs + (at[mb] % a.heads) * D;
+            meet_odd<TQ, TC, D>(a, s, g, odd_lo, odd_hi, N, N * WAVES, end, qp, sees[mb], m[mb], [&](const TC* v, bool seen, auto value, auto probability) {
+                bool any = false;
+#pragma unroll
+                for (int t = 0; t < DT; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) any |= !(fabsf(value(v + column<F32C>(t, p, e))) < __builtin_huge_valf());
+                if (!any || !seen) return;
+                const float y = probability();
+#pragma unroll
+                for (int t = 0; t < DT; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float x = value(v + column<F32C>(t, p, e));
+                        if (!(fabsf(x) < __builtin_huge_valf())) acc[mb][t][e] = fmaf(y, x, acc[mb][t][e]);
+                    }
+            });
+        }
     }
 
     // the waves' parts together

@@ -12,6 +12,8 @@
 // +- 32, and the rescaling of O none.  V is read transposed (ds_read_tr).
 // f32 pages: 32 x 32 x 2 products on float32 operands.  f32 rows over bf16
 // pages: three bf16 terms of q and p each, as in paged_few.hip.
+#include <type_traits>
+
 #include "paged_attn.h"
 
 namespace lq8 {
@@ -57,68 +59,131 @@ __device__ __forceinline__ bool find_tile(const AttnArgs& a, int want, int* span
     return *span >= 0;
 }
 
-template <int TYPES, int D, bool PREFIX>
-__global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
-    constexpr bool F32C = TYPES == PT_F32_F32, F32Q = TYPES != PT_BF16_BF16;
-    constexpr int TERMS = TYPES == PT_F32_BF16 ? 3 : 1;
-    constexpr int ES = F32C ? 4 : 2, ROW = D * ES, N = F32C ? 32 : 64;
-    constexpr int BLOCKS = N / 16, SB = N / 32;               // page blocks, score blocks of a tile
-    constexpr int CPR = ROW / 16, CI = N * CPR / THREADS;     // 16-byte chunks of a row; of a thread
-    constexpr int DT = D / 32, VW = D / 32;
-    __shared__ __attribute__((aligned(16))) char sk[2][N * ROW], sv[2][N * ROW];
-    __shared__ float scratch[4][16 * 32];
-    __shared__ int odd_tile[2];
+// A workgroup's rows and positions.
+struct Work {
+    Span s;
+    int g, piece, row0, packed, beg, end;
+};
+// Workgroup -> (row tile, piece, kv head), kv head fastest (one to an XCD where
+// there are eight); a sequence's last rows, which see most, first.  false:
+// nothing to do.
+template <bool PREFIX>
+__device__ __forceinline__ bool find_work(const AttnArgs& a, Work* k) {
+    const Cut& cut = PREFIX ? a.pre : a.own;
+    const int kvh = a.kv.kv_heads, x = blockIdx.x / kvh;
+    k->g = blockIdx.x % kvh;
+    k->piece = x % cut.pieces;
+    int sp, tile;
+    if (!find_tile<PREFIX>(a, x / cut.pieces, &sp, &tile)) return false;
+    k->s = PREFIX ? prefix_span(a, sp) : own_span(a, sp);
+    const int rows = k->s.count * a.group;
+    k->row0 = ((rows + TILE_PACKED - 1) / TILE_PACKED - 1 - tile) * TILE_PACKED;
+    k->packed = min(rows - k->row0, TILE_PACKED);
+    const int len = piece_len(k->s.length, cut), most = k->s.sees((k->row0 + k->packed - 1) / a.group);
+    k->beg = k->piece * len;
+    k->end = min(k->beg + len, most);
+    return a.part ? k->beg < most : k->piece == 0;
+}
+
+// A lane's row, and what it and its wave see.
+struct LaneRow {
+    bool valid, whole;  // whole: no spare rows in the wave (they are masked throughout)
+    int row, head, sees, least, most;
+    __device__ __forceinline__ LaneRow(const AttnArgs& a, const Work& k, int w, int r) {
+        const int G = a.group, first = k.row0 + 32 * w, pr = first + r, i = pr / G, end = k.row0 + k.packed;
+        const int last = min(first + 31, end - 1);
+        valid = pr < end;
+        whole = last == first + 31;
+        row = k.s.first + (valid ? i : 0);
+        head = k.g * G + (valid ? pr - i * G : 0);
+        sees = valid ? k.s.sees(i) : 0;
+        least = k.s.sees(first / G);
+        most = last < first ? 0 : k.s.sees(last / G);
+    }
+};
+
+// Results of a lane: piece's (o, m, l), or o / l.  m = -inf: nothing seen.
+template <bool F32, int D, bool PREFIX, typename F>
+__device__ __forceinline__ void finish(const AttnArgs& a, const Work& k, const LaneRow& me, int p, float m, float l, F put_all) {
+    l += lane_xor<32>(l);
+    if (!me.valid) return;
+    const bool none = m == -__builtin_huge_valf();
+    const size_t oat = me.row * a.os + (size_t)me.head * D;
+    if (a.part) {
+        const size_t slot = k.piece + (PREFIX ? a.own.pieces : 0), at = (slot * a.batch.rows + me.row) * a.heads + me.head;
+        if (p == 0) a.ml[at] = make_float2(m, l);
+        float* po = a.part + at * D;
+        put_all([&](int d, v4f y) { *(v4f*)(po + d) = none ? v4f{0, 0, 0, 0} : y; });
+    } else {
+        const float f = 1.0f / l;
+        put_all([&](int d, v4f y) {
+            y = none ? v4f{0, 0, 0, 0} : y * f;
+            if constexpr (F32) *(v4f*)((float*)a.out + oat + d) = y;
+            else *(uint2*)((uint16_t*)a.out + oat + d) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+        });
+    }
+}
+
+// meet_odd for a lane's sums; column(t, e): the head dimension of acc[t][e].
+template <typename T, typename C, int D, typename F>
+__device__ __forceinline__ void meet_odd_tile(const AttnArgs& a, const Work& k, const LaneRow& me, size_t qat, int lo, int hi, float m,
+                                              F column, v16f (&acc)[D / 32]) {
+    meet_odd<T, C, D>(a, k.s, k.g, lo, hi, hi - lo, hi - lo, min(hi, k.end), (const T*)a.q + qat, me.sees, m,
+                      [&](const C* v, bool seen, auto value, auto probability) {
+        bool any = false;
+#pragma unroll
+        for (int t = 0; t < D / 32; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) any |= !(fabsf(value(v + column(t, e))) < __builtin_huge_valf());
+        if (!any || !seen) return;
+        const float y = probability();
+#pragma unroll
+        for (int t = 0; t < D / 32; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const float x = value(v + column(t, e));
+                if (!(fabsf(x) < __builtin_huge_valf())) acc[t][e] = fmaf(y, x, acc[t][e]);
+            }
+    });
+}
+
+// The running reference of a row's exponents.  It follows the largest score
+// only when that passes it by 2^8 (somewhere in the wave): any reference gives
+// the same quotients, and the sums are rescaled a few times instead of often.
+constexpr float LAG = 8.0f;
+
+template <int TERMS, int D, bool PREFIX>
+__global__ __launch_bounds__(THREADS, 2) void k_tile_bf16(AttnArgs a) {
+    constexpr bool F32Q = TERMS > 1;
+    constexpr bool AHEAD = TERMS == 1;  // the next tile's scores are computed with this tile's probabilities
+    constexpr int ROW = 2 * D, N = 64, BLOCKS = N / 16, SB = N / 32;
+    constexpr int CI = N * ROW / (THREADS * 16);  // 1 KiB loads of a wave, K or V
+    constexpr int DT = D / 32, KS = D / 16;
+    constexpr int VR = TERMS == 1 ? 5 : 3;                // V operands in registers
+    constexpr int TB = N * ROW;  // bytes of a tile's K or V; in LDS K of two tiles, then V of two
+    __shared__ __attribute__((aligned(256))) char sm[4 * TB];
+    __shared__ int odd_lo, odd_hi;  // positions of tiles with values that are not finite
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, p = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    Work wk;
+    if (!find_work<PREFIX>(a, &wk)) return;
+    const Span& s = wk.s;
+    const int g = wk.g, beg = wk.beg, end = wk.end;
+    if (tid == 0) odd_lo = INT32_MAX, odd_hi = 0;
+    const LaneRow me(a, wk, w, r);
+    const size_t qat = me.row * a.qs + (size_t)me.head * D;
 
-    // workgroup -> (row tile, piece, kv head), kv head fastest (one to an XCD
-    // where there are eight); a sequence's last rows, which see most, first
-    const int G = a.group, kvh = a.kv.kv_heads;
-    const Cut& cut = PREFIX ? a.pre : a.own;
-    int x = blockIdx.x;
-    const int g = x % kvh;
-    x /= kvh;
-    const int piece = x % cut.pieces, want = x / cut.pieces;
-    int sp, tile;
-    if (!find_tile<PREFIX>(a, want, &sp, &tile)) return;
-    const Span s = PREFIX ? prefix_span(a, sp) : own_span(a, sp);
-    tile = (s.count * G + TILE_PACKED - 1) / TILE_PACKED - 1 - tile;
-    const int row0 = tile * TILE_PACKED, packed = min(s.count * G - row0, TILE_PACKED);
-    const int len = piece_len(s.length, cut);
-    const int most = s.sees((row0 + packed - 1) / G);
-    const int beg = piece * len, end = min(beg + len, most);
-    if (a.part ? beg >= most : piece > 0) return;
-    if (tid < 2) odd_tile[tid] = -1;
-
-    // the lane's row
-    const int wrow = row0 + 32 * w, pr = wrow + r, i = pr / G;
-    const bool valid = pr < row0 + packed;
-    const int row = s.first + (valid ? i : 0), head = g * G + (valid ? pr - i * G : 0);
-    const int sees = valid ? s.sees(i) : 0;
-    const int wleast = s.sees(wrow / G), wlast = min(wrow + 31, row0 + packed - 1);
-    const int wmost = wlast < wrow ? 0 : s.sees(wlast / G);
-    const bool whole = wlast == wrow + 31;  // (a wave with spare rows masks them throughout)
-    const size_t qat = row * a.qs + (size_t)head * D;
-    uint32_t q[F32C ? 1 : TERMS][F32C ? 1 : D / 16][4];
-    float qf[F32C ? D / 2 : 1];
-    if constexpr (F32C) {
-        const float* qp = (const float*)a.q + qat + 4 * p;
-#pragma unroll
-        for (int t = 0; t < D / 8; t++) {
-            const float4 v = *(const float4*)(qp + 8 * t);
-            qf[4 * t] = v.x, qf[4 * t + 1] = v.y, qf[4 * t + 2] = v.z, qf[4 * t + 3] = v.w;
-        }
-    } else if constexpr (F32Q) {
+    v4u q[TERMS][KS];
+    if constexpr (F32Q) {
         const float* qp = (const float*)a.q + qat + 8 * p;
 #pragma unroll
-        for (int t = 0; t < D / 16; t++) {
-            const float4 y0 = *(const float4*)(qp + 16 * t), y1 = *(const float4*)(qp + 16 * t + 4);
-            const float y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
+        for (int t = 0; t < KS; t++) {
+            const v4f y0 = *(const v4f*)(qp + 16 * t), y1 = *(const v4f*)(qp + 16 * t + 4);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 float t0[3], t1[3];
-                three_terms(y[2 * e], t0);
-                three_terms(y[2 * e + 1], t1);
+                three_terms(e < 2 ? y0[2 * e] : y1[2 * e - 4], t0);
+                three_terms(e < 2 ? y0[2 * e + 1] : y1[2 * e - 3], t1);
 #pragma unroll
                 for (int z = 0; z < TERMS; z++) q[z][t][e] = pack_bf16(t0[z], t1[z]);
             }
@@ -126,9 +191,306 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
     } else {
         const uint16_t* qp = (const uint16_t*)a.q + qat + 8 * p;
 #pragma unroll
-        for (int t = 0; t < D / 16; t++) {
-            const v4u v = *(const v4u*)(qp + 16 * t);
-            q[0][t][0] = v[0], q[0][t][1] = v[1], q[0][t][2] = v[2], q[0][t][3] = v[3];
+        for (int t = 0; t < KS; t++) q[0][t] = *(const v4u*)(qp + 16 * t);
+    }
+
+    v16f acc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[t][e] = 0.0f;
+    float m = -__builtin_huge_valf(), l = 0.0f;
+
+    // Tiles go from the cache to LDS without registers (16 bytes a lane, lane
+    // order in LDS): the lane loads the chunk that lds_slot puts at its place.
+    const char *kc = (const char*)a.kv.k, *vc = (const char*)a.kv.v;
+    unsigned lane_src;
+    int lane_row;  // byte offset inside its 16-row block; row inside its wave's 1 KiB of the tile
+    {
+        const int sub = lane >> 4;
+        if constexpr (ROW == 256) {
+            lane_row = sub;
+            lane_src = (4 * w + sub) * ROW + (((lane & 15) ^ ((sub << 2) | w)) << 4);
+        } else {
+            const int x = (lane & 15) ^ (((sub & 1) << 2) | ((2 * w + (sub >> 1)) & 3));
+            lane_row = 2 * sub + (x >> 3);
+            lane_src = ((8 * w + lane_row) & 15) * ROW + ((x & 7) << 4);
+        }
+    }
+    constexpr int WROWS = 1024 / ROW;  // rows of a wave's load
+    auto page_of = [&](const int (&pg)[BLOCKS], int n) {
+        if constexpr (ROW == 256) return pg[n];
+        else return w >= 2 ? pg[2 * n + 1] : pg[2 * n];
+    };
+    auto fetch = [&](const char* from, char* to, const int (&pg)[BLOCKS], int j) {
+        typedef __attribute__((address_space(3))) void* LP;
+        typedef const __attribute__((address_space(1))) void* GP;
+#pragma unroll
+        for (int n = 0; n < CI; n++) {
+            const int row = (4 * n + w) * WROWS;
+            const char* src = from + slot_off(a, page_of(pg, n), g, j + (row & ~15), D) * 2;
+            __builtin_amdgcn_global_load_lds((GP)(src + lane_src), (LP)(to + (4 * n + w) * 1024), 16, 0, 0);
+        }
+    };
+    auto pages_of = [&](int j, int (&pg)[BLOCKS]) {
+#pragma unroll
+        for (int b = 0; b < BLOCKS; b++) pg[b] = page_at(a, s, j + 16 * b, end);
+    };
+    // Values of rows that no row sees become zeros, and so does what is not
+    // finite where some row must not meet it (three terms: anywhere); each
+    // lane looks after the chunks it has loaded.
+    const int least = s.sees(wk.row0 / a.group);
+    auto mend = [&](char* V, const int (&pg)[BLOCKS], int j) {
+        bool hole = false;
+#pragma unroll
+        for (int b = 0; b < BLOCKS; b++) hole |= pg[b] < 0;
+        const bool part = hole || j + N > least;
+        if (!part && TERMS == 1) return;
+        uint32_t bits = 0;
+        v4u v[CI];
+#pragma unroll
+        for (int n = 0; n < CI; n++) {
+            v4u* at = (v4u*)(V + (4 * n + w) * 1024 + 16 * lane);
+            v[n] = *at;
+            if (part && (page_of(pg, n) < 0 || j + (4 * n + w) * WROWS + lane_row >= end)) {
+                v[n] = v4u{0, 0, 0, 0};
+                *at = v[n];
+            }
+            mark_odd<false>(v[n], bits);
+        }
+        if (is_odd<false>(bits)) {
+            atomicMin(&odd_lo, j);
+            atomicMax(&odd_hi, j + N);
+#pragma unroll
+            for (int n = 0; n < CI; n++) *(v4u*)(V + (4 * n + w) * 1024 + 16 * lane) = finite_part<false>(v[n]);
+        }
+    };
+    // Scores of a tile, K's operands two steps ahead; beside(c): other work
+    // that goes between the products of step c, which keep the order written
+    // (left alone, the compiler loads all operands first and spills).
+    auto scores = [&](int K, v16f (&sc)[SB], auto beside) {
+        // lds_slot(32 b + r, 2 c + p) = (lds_slot(r, p) ^ 32 c) + 32 b ROW, from
+        // one register (hoisted out of the loop the places take eight)
+        int at = K + lds_slot<ROW>(r, p);
+        asm volatile("" : "+v"(at));
+        v8b ko[3][SB];
+        auto load = [&](int c) {
+#pragma unroll
+            for (int b = 0; b < SB; b++) ko[c % 3][b] = *(const v8b*)(sm + ((at ^ (c << 5)) + 32 * b * ROW));
+        };
+        load(0);
+        load(1);
+#pragma unroll
+        for (int b = 0; b < SB; b++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) sc[b][e] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < KS; c++) {
+            if (c + 2 < KS) load(c + 2);
+#pragma unroll
+            for (int z = TERMS - 1; z >= 0; z--)
+#pragma unroll
+                for (int b = 0; b < SB; b++)
+                    sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ko[c % 3][b], __builtin_bit_cast(v8b, q[z][c]), sc[b], 0, 0, 0);
+            beside(c);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto nothing = [](int) {};
+
+    int pg[BLOCKS], p1[BLOCKS], p2[BLOCKS];  // pages of this tile and the next two
+    int j = beg;
+    if (j < end) {
+        pages_of(j, pg);
+        pages_of(j + N, p1);
+        pages_of(j + 2 * N, p2);
+        fetch(kc, sm, pg, j);
+        fetch(vc, sm + 2 * TB, pg, j);
+        if (AHEAD && j + N < end) fetch(kc, sm + TB, p1, j + N);
+#pragma unroll
+        for (int z = 0; z < TERMS; z++)
+#pragma unroll
+            for (int t = 0; t < KS; t++) arrived(q[z][t]);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();  // odd_lo, odd_hi are set up
+        mend(sm + 2 * TB, pg, j);
+        __syncthreads();
+    }
+    v16f sc[SB];
+    if (AHEAD && j < end && j < me.most) scores(0, sc, nothing);
+    for (int k = 0; j < end; k++, j += N) {
+        const int buf = k & 1, jn = j + N;
+        if (AHEAD) {
+            if (jn + N < end) fetch(kc, sm + buf * TB, p2, jn + N);
+            if (jn < end) fetch(vc, sm + (2 + (buf ^ 1)) * TB, p1, jn);
+        } else if (jn < end) {
+            fetch(kc, sm + (buf ^ 1) * TB, p1, jn);
+            fetch(vc, sm + (2 + (buf ^ 1)) * TB, p1, jn);
+        }
+        int p3[BLOCKS];
+        pages_of(jn + 2 * N, p3);
+        if (j < me.most) {
+            if (!AHEAD) scores(buf * TB, sc, nothing);
+            bool hole = false;
+#pragma unroll
+            for (int b = 0; b < BLOCKS; b++) hole |= pg[b] < 0;
+            const bool masked = hole || j + N > me.least || !me.whole;
+            // element e of block b: position 32 b + 8 (e / 4) + 4 p + e % 4
+            float mx = -FLT_MAX;
+            if (masked) {
+                mx = -__builtin_huge_valf();
+#pragma unroll
+                for (int b = 0; b < SB; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const bool seen = pg[2 * b + e / 8] >= 0 && j + 32 * b + 8 * (e / 4) + 4 * p + e % 4 < me.sees;
+                        sc[b][e] = seen ? sc[b][e] : -__builtin_huge_valf();
+                        mx = seen ? -FLT_MAX : mx;
+                    }
+            }
+            if constexpr (TERMS > 1) {
+                // an infinity times the terms of a q may be inf - inf: such scores again, product by product
+                float sum = 0.0f;
+#pragma unroll
+                for (int b = 0; b < SB; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) sum += sc[b][e];
+                if (__any(sum != sum)) {
+#pragma unroll
+                    for (int b = 0; b < SB; b++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++)
+                            if (sc[b][e] != sc[b][e]) {
+                                const float* qp = (const float*)a.q + qat;
+                                const uint16_t* kp = (const uint16_t*)kc + slot_off(a, pg[2 * b + e / 8], g, j + 32 * b + 16 * (e / 8), D) +
+                                                     (8 * (e / 4 % 2) + 4 * p + e % 4) * D;
+                                float t = 0.0f;
+                                for (int d = 0; d < D; d++) t = fmaf(qp[d], __uint_as_float((uint32_t)kp[d] << 16), t);
+                                sc[b][e] = t;
+                            }
+                }
+            }
+            {
+                // (c > 0: the largest score scaled is the largest scaled score)
+                float y = sc[0][0];
+#pragma unroll
+                for (int b = 0; b < SB; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) y = fmaxf(y, sc[b][e]);
+                mx = fmaxf(mx, y * a.c);
+            }
+            mx = fmaxf(mx, lane_xor<32>(mx));
+            if (__any(mx > m + LAG)) {
+                const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - fmaxf(mn, -FLT_MAX));
+                l *= al;
+#pragma unroll
+                for (int t = 0; t < DT; t++) acc[t] *= al;
+                m = mn;
+            }
+            float mu = fmaxf(m, -FLT_MAX), c = a.c;
+            if (__any(far_score(mu))) {
+#pragma unroll
+                for (int b = 0; b < SB; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) sc[b][e] = sc[b][e] * c - mu;
+                c = 1.0f, mu = 0.0f;
+            }
+            // probabilities e0 .. e0 + n - 1 of the tile's 32, in place
+            auto probabilities = [&](int e0, int n) {
+#pragma unroll
+                for (int e = e0; e < e0 + n; e++) {
+                    const float y = __builtin_amdgcn_exp2f(fmaf(sc[e / 16][e % 16], c, -mu));
+                    sc[e / 16][e % 16] = y;
+                    l += y;
+                }
+            };
+            v16f nx[SB];
+            if (AHEAD && jn < end && jn < me.most) scores((buf ^ 1) * TB, nx, [&](int step) { probabilities(step * (32 / KS), 32 / KS); });
+            else probabilities(0, 32);
+            // lds_slot(16 ks + 8 h + row, ch + 4 t) = (lds_slot(row, ch) ^ 64 t ^ 32 h) + (16 ks + 8 h) ROW
+            int vat = (2 + buf) * TB + lds_slot<ROW>(4 * p + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 8 * (lane & 1);
+            asm volatile("" : "+v"(vat));
+            v8b vo[VR];
+            auto load_v = [&](int i) {
+                const int ks = i / DT, t = i % DT;
+                const char* at = sm + 16 * ks * ROW;
+                vo[i % VR] = join_halves(read_transposed(at + (vat ^ (t << 6))), read_transposed(at + 8 * ROW + (vat ^ (t << 6) ^ 32)));
+            };
+#pragma unroll
+            for (int i = 0; i + 1 < VR; i++) load_v(i);
+#pragma unroll
+            for (int ks = 0; ks < N / 16; ks++) {
+                v4u pb[TERMS];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float y0 = sc[ks / 2][8 * (ks % 2) + 2 * e], y1 = sc[ks / 2][8 * (ks % 2) + 2 * e + 1];
+                    if constexpr (TERMS == 1) {
+                        pb[0][e] = pack_bf16(y0, y1);
+                    } else {
+                        float t0[3], t1[3];
+                        three_terms(y0, t0);
+                        three_terms(y1, t1);
+#pragma unroll
+                        for (int z = 0; z < TERMS; z++) pb[z][e] = pack_bf16(t0[z], t1[z]);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < DT; t++) {
+                    const int i = ks * DT + t;
+                    if (i + VR - 1 < N / 16 * DT) load_v(i + VR - 1);
+#pragma unroll
+                    for (int z = TERMS - 1; z >= 0; z--)
+                        acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vo[i % VR], __builtin_bit_cast(v8b, pb[z]), acc[t], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if (AHEAD) {
+#pragma unroll
+                for (int b = 0; b < SB; b++) sc[b] = nx[b];
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the fetches)
+        if (jn < end) mend(sm + (2 + (buf ^ 1)) * TB, p1, jn);
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < BLOCKS; b++) pg[b] = p1[b], p1[b] = p2[b], p2[b] = p3[b];
+    }
+    __syncthreads();
+    if (odd_hi) meet_odd_tile<typename std::conditional<F32Q, float, uint16_t>::type, uint16_t, D>(a, wk, me, qat, odd_lo, odd_hi, m, [&](int t, int e) { return 32 * t + 8 * (e / 4) + 4 * p + e % 4; }, acc);
+    finish<F32Q, D, PREFIX>(a, wk, me, p, m, l, [&](auto put) {
+#pragma unroll
+        for (int t = 0; t < DT; t++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) put(32 * t + 2 * e + 4 * p, v4f{acc[t][e], acc[t][e + 1], acc[t][e + 2], acc[t][e + 3]});
+    });
+}
+
+template <int D, bool PREFIX>
+__global__ __launch_bounds__(THREADS, 2) void k_tile_f32(AttnArgs a) {
+    constexpr int ES = 4, ROW = D * ES, N = 32;
+    constexpr int BLOCKS = N / 16, SB = N / 32;               // page blocks, score blocks of a tile
+    constexpr int CPR = ROW / 16, CI = N * CPR / THREADS;     // 16-byte chunks of a row; of a thread
+    constexpr int DT = D / 32, VW = D / 32;
+    __shared__ __attribute__((aligned(16))) char sk[2][N * ROW], sv[2][N * ROW];
+    __shared__ int odd_lo, odd_hi;  // positions of tiles with values that are not finite
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, p = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+    Work wk;
+    if (!find_work<PREFIX>(a, &wk)) return;
+    const Span& s = wk.s;
+    const int g = wk.g, beg = wk.beg, end = wk.end;
+    if (tid == 0) odd_lo = INT32_MAX, odd_hi = 0;
+    const LaneRow me(a, wk, w, r);
+    const size_t qat = me.row * a.qs + (size_t)me.head * D;
+    float qf[D / 2];
+    {
+        const float* qp = (const float*)a.q + qat + 4 * p;
+#pragma unroll
+        for (int t = 0; t < D / 8; t++) {
+            const v4f v = *(const v4f*)(qp + 8 * t);
+#pragma unroll
+            for (int e = 0; e < 4; e++) qf[4 * t + e] = v[e];
         }
     }
 
@@ -163,26 +525,27 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
             vr[n] = *(const v4u*)(vc + at + o);
         }
     };
-    // registers -> buffer `buf`, tile number k at position j.  Values of rows
+    // registers -> buffer `buf`, the tile at position j.  Values of rows
     // that no row sees become zeros, and so does what is not finite where
     // some row must not meet it (fixed up after the products).
-    const int least = s.sees(row0 / G);
-    auto store = [&](int buf, int k, int j, const int (&pg)[BLOCKS]) {
+    const int least = s.sees(wk.row0 / a.group);
+    auto store = [&](int buf, int j, const int (&pg)[BLOCKS]) {
         bool hole = false;
 #pragma unroll
         for (int b = 0; b < BLOCKS; b++) hole |= pg[b] < 0;
-        const bool check = TERMS > 1 || hole || j + N > least;
+        const bool check = hole || j + N > least;
         if (check) {
             uint32_t bits = 0;
 #pragma unroll
             for (int n = 0; n < CI; n++) {
                 if (page_of(pg, n) < 0 || j + n * RPN + tid / CPR >= end) vr[n] = v4u{0, 0, 0, 0};
-                mark_odd<F32C>(vr[n], bits);
+                mark_odd<true>(vr[n], bits);
             }
-            if (is_odd<F32C>(bits)) {
-                odd_tile[buf] = k;
+            if (is_odd<true>(bits)) {
+                atomicMin(&odd_lo, j);
+                atomicMax(&odd_hi, j + N);
 #pragma unroll
-                for (int n = 0; n < CI; n++) vr[n] = finite_part<F32C>(vr[n]);
+                for (int n = 0; n < CI; n++) vr[n] = finite_part<true>(vr[n]);
             }
         }
 #pragma unroll
@@ -198,92 +561,44 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
         pages_of(j, pg);
         pages_of(j + N, pn);
         load(pg, j);
-        __syncthreads();  // odd_tile is set up
-        store(0, 0, j, pg);
+        __syncthreads();  // odd_lo, odd_hi are set up
+        store(0, j, pg);
     }
-    if constexpr (F32C) {
 #pragma unroll
-        for (int t = 0; t < D / 2; t++) arrived(qf[t]);
-    } else {
-#pragma unroll
-        for (int z = 0; z < TERMS; z++)
-#pragma unroll
-            for (int t = 0; t < D / 16; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) arrived(q[z][t][e]);
-    }
+    for (int t = 0; t < D / 2; t++) arrived(qf[t]);
     for (int k = 0; j < end; k++, j += N) {
         const int buf = k & 1, jn = j + N;
         __syncthreads();
         if (jn < end) load(pn, jn);
         int pnn[BLOCKS];  // a tile ahead of its loads
         pages_of(jn + N, pnn);
-        if (j < wmost) {
+        if (j < me.most) {
             const char *K = sk[buf], *V = sv[buf];
             v16f sc[SB];
-            v8b ko[F32C ? 1 : SB][F32C ? 1 : D / 16];
-            if constexpr (!F32C) {
-#pragma unroll
-                for (int b = 0; b < SB; b++)
-#pragma unroll
-                    for (int c = 0; c < D / 16; c++) ko[b][c] = *(const v8b*)(K + lds_slot<ROW>(32 * b + r, 2 * c + p));
-            }
 #pragma unroll
             for (int b = 0; b < SB; b++) {
                 v16f t;
 #pragma unroll
                 for (int e = 0; e < 16; e++) t[e] = 0.0f;
-                if constexpr (F32C) {
 #pragma unroll
-                    for (int c = 0; c < D / 8; c++) {
-                        const v4f kv = *(const v4f*)(K + lds_slot<ROW>(32 * b + r, 2 * c + p));
+                for (int c = 0; c < D / 8; c++) {
+                    const v4f kv = *(const v4f*)(K + lds_slot<ROW>(32 * b + r, 2 * c + p));
 #pragma unroll
-                        for (int e = 0; e < 4; e++) t = __builtin_amdgcn_mfma_f32_32x32x2f32(kv[e], qf[4 * c + e], t, 0, 0, 0);
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < D / 16; c++) {
-#pragma unroll
-                        for (int z = TERMS - 1; z >= 0; z--) {
-                            const v4u qv = v4u{q[z][c][0], q[z][c][1], q[z][c][2], q[z][c][3]};
-                            t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ko[b][c], __builtin_bit_cast(v8b, qv), t, 0, 0, 0);
-                        }
-                    }
+                    for (int e = 0; e < 4; e++) t = __builtin_amdgcn_mfma_f32_32x32x2f32(kv[e], qf[4 * c + e], t, 0, 0, 0);
                 }
                 sc[b] = t;
             }
             bool hole = false;
 #pragma unroll
             for (int b = 0; b < BLOCKS; b++) hole |= pg[b] < 0;
-            const bool masked = hole || j + N > wleast || !whole;
+            const bool masked = hole || j + N > me.least || !me.whole;
             // element e of block b: position 32 b + 8 (e / 4) + 4 p + e % 4
-            auto seen = [&](int b, int e) { return pg[2 * b + e / 8] >= 0 && j + 32 * b + 8 * (e / 4) + 4 * p + e % 4 < sees; };
+            auto seen = [&](int b, int e) { return pg[2 * b + e / 8] >= 0 && j + 32 * b + 8 * (e / 4) + 4 * p + e % 4 < me.sees; };
             if (masked) {
 #pragma unroll
                 for (int b = 0; b < SB; b++)
 #pragma unroll
                     for (int e = 0; e < 16; e++) sc[b][e] = seen(b, e) ? sc[b][e] : -__builtin_huge_valf();
-            }
-            if constexpr (TERMS > 1) {
-                // an infinity times the terms of a q may be inf - inf: such scores again, product by product
-                float sum = 0.0f;
-#pragma unroll
-                for (int b = 0; b < SB; b++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) sum += sc[b][e];
-                if (__any(sum != sum)) {
-#pragma unroll
-                    for (int b = 0; b < SB; b++)
-#pragma unroll
-                        for (int e = 0; e < 16; e++)
-                            if (sc[b][e] != sc[b][e]) {
-                                const float* qp = (const float*)a.q + qat;
-                                const uint16_t* kp = (const uint16_t*)kc + slot_off(a, pg[2 * b + e / 8], g, j + 32 * b + 16 * (e / 8), D) + (8 * (e / 4 % 2) + 4 * p + e % 4) * D;
-                                float t = 0.0f;
-                                for (int d = 0; d < D; d++) t = fmaf(qp[d], __uint_as_float((uint32_t)kp[d] << 16), t);
-                                sc[b][e] = t;
-                            }
-                }
             }
             float mx = masked ? -__builtin_huge_valf() : -FLT_MAX;
             if (masked) {
@@ -331,7 +646,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
                     sc[b][e] = __builtin_amdgcn_exp2f(sc[b][e]);
                     l += sc[b][e];
                 }
-            if constexpr (F32C) {
+            {
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     const int vrow = 8 * (e / 4) + 4 * p + e % 4;
@@ -345,109 +660,39 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile(AttnArgs a) {
 #pragma unroll
                     for (int t = 0; t < DT; t++) acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[t], sc[0][e], acc[t], 0, 0, 0);
                 }
-            } else {
-#pragma unroll
-                for (int ks = 0; ks < N / 16; ks++) {
-                    uint32_t pb[TERMS][4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float y0 = sc[ks / 2][8 * (ks % 2) + 2 * e], y1 = sc[ks / 2][8 * (ks % 2) + 2 * e + 1];
-                        if constexpr (TERMS == 1) {
-                            pb[0][e] = pack_bf16(y0, y1);
-                        } else {
-                            float t0[3], t1[3];
-                            three_terms(y0, t0);
-                            three_terms(y1, t1);
-#pragma unroll
-                            for (int z = 0; z < TERMS; z++) pb[z][e] = pack_bf16(t0[z], t1[z]);
-                        }
-                    }
-                    const int i16 = lane & 15, dh = (lane >> 4) & 1;
-                    const int vrow = 16 * ks + 4 * p + (i16 >> 2), ch = 2 * dh + ((i16 >> 1) & 1), in = 8 * (i16 & 1);
-#pragma unroll
-                    for (int t = 0; t < DT; t++) {
-                        const v8b va = join_halves(read_transposed(V + lds_slot<ROW>(vrow, ch + 4 * t) + in),
-                                                   read_transposed(V + lds_slot<ROW>(vrow + 8, ch + 4 * t) + in));
-#pragma unroll
-                        for (int z = TERMS - 1; z >= 0; z--) {
-                            const v4u pv = v4u{pb[z][0], pb[z][1], pb[z][2], pb[z][3]};
-                            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, __builtin_bit_cast(v8b, pv), acc[t], 0, 0, 0);
-                        }
-                    }
-                }
-            }
-            if (odd_tile[buf] == k) {
-                // the values that are not finite, for the rows that see them
-                float* ps = scratch[w];
-#pragma unroll
-                for (int b = 0; b < BLOCKS; b++) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) ps[(8 * (e / 4) + 4 * p + e % 4) * 32 + r] = sc[b / 2][8 * (b % 2) + e];
-                    __builtin_amdgcn_wave_barrier();
-                    const size_t from = slot_off(a, pg[b], g, j + 16 * b, D);
-                    for (int jj = 0; jj < 16 && pg[b] >= 0 && j + 16 * b + jj < end; jj++) {
-                        const float y = ps[jj * 32 + r];
-                        const bool see = j + 16 * b + jj < sees;
-#pragma unroll
-                        for (int t = 0; t < DT; t++)
-#pragma unroll
-                            for (int e = 0; e < 16; e++) {
-                                const int mrow = 8 * (e / 4) + 4 * p + e % 4;
-                                float v;
-                                if constexpr (F32C) v = ((const float*)vc)[from + jj * D + VW * mrow + t];
-                                else v = __uint_as_float((uint32_t)((const uint16_t*)vc)[from + jj * D + 32 * t + mrow] << 16);
-                                if (!(fabsf(v) < __builtin_huge_valf()) && see) acc[t][e] = fmaf(y, v, acc[t][e]);
-                            }
-                    }
-                    __builtin_amdgcn_wave_barrier();
-                }
             }
         }
-        if (jn < end) store(buf ^ 1, k + 1, jn, pn);
+        if (jn < end) store(buf ^ 1, jn, pn);
 #pragma unroll
         for (int b = 0; b < BLOCKS; b++) pg[b] = pn[b], pn[b] = pnn[b];
     }
 
-    l += lane_xor<32>(l);
-    if (!valid) return;
-    const bool none = m == -__builtin_huge_valf();
-    float f = none ? 0.0f : 1.0f / l;
-    float* po = nullptr;
-    if (a.part) {
-        const size_t slot = piece + (PREFIX ? a.own.pieces : 0), k = (slot * a.batch.rows + row) * a.heads + head;
-        if (p == 0) a.ml[k] = make_float2(m, l);
-        po = a.part + k * D;
-        f = 1.0f;
-    }
-    const size_t oat = row * a.os + (size_t)head * D;
-    auto put = [&](int d, v4f y) {
-        y = none ? v4f{0, 0, 0, 0} : y * f;
-        if (a.part) *(v4f*)(po + d) = y;
-        else if constexpr (F32Q) *(v4f*)((float*)a.out + oat + d) = y;
-        else *(uint2*)((uint16_t*)a.out + oat + d) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
-    };
-    if constexpr (!F32C) {
+    __syncthreads();
+    if (odd_hi) meet_odd_tile<float, float, D>(a, wk, me, qat, odd_lo, odd_hi, m, [&](int t, int e) { return VW * (8 * (e / 4) + 4 * p + e % 4) + t; }, acc);
+    finish<true, D, PREFIX>(a, wk, me, p, m, l, [&](auto put) {
+        if constexpr (VW == 4) {
 #pragma unroll
-        for (int t = 0; t < DT; t++)
+            for (int e = 0; e < 16; e++)
+                put(4 * (8 * (e / 4) + 4 * p + e % 4), v4f{acc[0][e], acc[1 % DT][e], acc[2 % DT][e], acc[3 % DT][e]});
+        } else {
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) put(32 * t + 2 * e + 4 * p, v4f{acc[t][e], acc[t][e + 1], acc[t][e + 2], acc[t][e + 3]});
-    } else if constexpr (VW == 4) {
-#pragma unroll
-        for (int e = 0; e < 16; e++)
-            put(4 * (8 * (e / 4) + 4 * p + e % 4), v4f{acc[0][e], acc[1 % DT][e], acc[2 % DT][e], acc[3 % DT][e]});
-    } else {
-#pragma unroll
-        for (int e = 0; e < 16; e += 2)
-            put(2 * (8 * (e / 4) + 4 * p + e % 4), v4f{acc[0][e], acc[1][e], acc[0][e + 1], acc[1][e + 1]});
-    }
+            for (int e = 0; e < 16; e += 2)
+                put(2 * (8 * (e / 4) + 4 * p + e % 4), v4f{acc[0][e], acc[1][e], acc[0][e + 1], acc[1][e + 1]});
+        }
+    });
 }
 
+template <int TYPES, int D, bool PREFIX>
+void launch_one(dim3 grid, hipStream_t s, const AttnArgs& a) {
+    if constexpr (TYPES == PT_F32_F32) hipLaunchKernelGGL((k_tile_f32<D, PREFIX>), grid, dim3(THREADS), 0, s, a);
+    else hipLaunchKernelGGL((k_tile_bf16<TYPES == PT_F32_BF16 ? 3 : 1, D, PREFIX>), grid, dim3(THREADS), 0, s, a);
+}
 template <int TYPES>
 void launch_types(dim3 grid, hipStream_t s, const AttnArgs& a, int dim, bool prefix) {
-    if (dim == 64 && prefix) hipLaunchKernelGGL((k_tile<TYPES, 64, true>), grid, dim3(THREADS), 0, s, a);
-    else if (dim == 64) hipLaunchKernelGGL((k_tile<TYPES, 64, false>), grid, dim3(THREADS), 0, s, a);
-    else if (prefix) hipLaunchKernelGGL((k_tile<TYPES, 128, true>), grid, dim3(THREADS), 0, s, a);
-    else hipLaunchKernelGGL((k_tile<TYPES, 128, false>), grid, dim3(THREADS), 0, s, a);
+    if (dim == 64 && prefix) launch_one<TYPES, 64, true>(grid, s, a);
+    else if (dim == 64) launch_one<TYPES, 64, false>(grid, s, a);
+    else if (prefix) launch_one<TYPES, 128, true>(grid, s, a);
+    else launch_one<TYPES, 128, false>(grid, s, a);
 }
 
 }  // namespace
