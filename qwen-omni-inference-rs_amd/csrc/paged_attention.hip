@@ -167,14 +167,14 @@ Plan plan_of(AttnArgs* a, PagedTypes types, int dim, int cus) {
     const size_t own = (size_t)a->batch.max_rows * G, each = (own + TILE_PACKED - 1) / TILE_PACKED;
     p.own_few = own <= FEW_MAX_ROWS;
     p.own_blocks = own <= 16 ? 1 : 2;
-    p.own_tiles = p.own_few ? batch : std::min(batch * each, rows * G / TILE_PACKED + std::min(batch, rows));
+    p.own_tiles = p.own_few ? batch : std::min(batch * each, (rows * G + (TILE_PACKED - 1) * std::min(batch, rows)) / TILE_PACKED);
     a->own = cut_of((size_t)a->batch.max_pages << a->kv.page_shift, p.own_tiles * kvh, cus, p.own_few, f32);
     p.slots = a->own.pieces;
     if (a->prefix.groups) {
         const size_t groups = a->prefix.groups;
         p.pre_few = rows * G <= FEW_MAX_ROWS;
         p.pre_blocks = rows * G <= 16 ? 1 : 2;
-        p.pre_tiles = p.pre_few ? groups : rows * G / TILE_PACKED + std::min(groups, rows);
+        p.pre_tiles = p.pre_few ? groups : (rows * G + (TILE_PACKED - 1) * std::min(groups, rows)) / TILE_PACKED;
         a->pre = cut_of((size_t)a->prefix.max_pages << a->kv.page_shift, p.pre_tiles * kvh, cus, p.pre_few, f32);
         p.slots += a->pre.pieces;
     }

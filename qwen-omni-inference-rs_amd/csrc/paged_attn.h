@@ -119,6 +119,11 @@ __device__ __forceinline__ void three_terms(float x, float (&t)[3]) {
     t[2] = r - t[1];
 }
 
+// both halves of w added to x
+__device__ __forceinline__ float add_bf16(uint32_t w, float x) {
+    typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2b, w), v2b{(__bf16)1.0f, (__bf16)1.0f}, x, false);
+}
 __device__ __forceinline__ v8b join_halves(v4s a, v4s b) {
     return __builtin_bit_cast(v8b, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }

@@ -138,12 +138,15 @@ __device__ __forceinline__ void meet_odd_tile(const AttnArgs& a, const Work& k, 
         if (!any || !seen) return;
         const float y = probability();
 #pragma unroll
-        for (int t = 0; t < D / 32; t++)
+        for (int t = 0; t < D / 32; t++) {
+            v16f add;
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 const float x = value(v + column(t, e));
-                if (!(fabsf(x) < __builtin_huge_valf())) acc[t][e] = fmaf(y, x, acc[t][e]);
+                add[e] = fabsf(x) < __builtin_huge_valf() ? 0.0f : y * x;
             }
+            acc[t] += add;  // (as whole vectors: single elements written here split the sums' registers in the main loop)
+        }
     });
 }
 
@@ -155,8 +158,7 @@ constexpr float LAG = 8.0f;
 template <int TERMS, int D, bool PREFIX>
 __global__ __launch_bounds__(THREADS, 2) void k_tile_bf16(AttnArgs a) {
     constexpr bool F32Q = TERMS > 1;
-    constexpr bool AHEAD = TERMS == 1;  // the next tile's scores are computed with this tile's probabilities
-    constexpr int ROW = 2 * D, N = 64, BLOCKS = N / 16, SB = N / 32;
+    constexpr int ROW = 2 * D, N = 64, SB = N / 32;
     constexpr int CI = N * ROW / (THREADS * 16);  // 1 KiB loads of a wave, K or V
     constexpr int DT = D / 32, KS = D / 16;
     constexpr int VR = TERMS == 1 ? 5 : 3;                // V operands in registers
@@ -218,41 +220,58 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile_bf16(AttnArgs a) {
         }
     }
     constexpr int WROWS = 1024 / ROW;  // rows of a wave's load
-    auto page_of = [&](const int (&pg)[BLOCKS], int n) {
-        if constexpr (ROW == 256) return pg[n];
-        else return w >= 2 ? pg[2 * n + 1] : pg[2 * n];
+    const unsigned long long klane = (unsigned long long)kc + lane_src, vlane = (unsigned long long)vc + lane_src;
+    // A tile's pages: lane l looks after block l % 4, whose slots lie `off`
+    // bytes into the cache (of page 0 where no page holds them).
+    struct Pages {
+        int id;
+        unsigned long long off;
     };
-    auto fetch = [&](const char* from, char* to, const int (&pg)[BLOCKS], int j) {
+    const unsigned bytes_in = (unsigned)g << a.kv.page_shift, slots = (1u << a.kv.page_shift) - 1;
+    const unsigned long long page_bytes = a.kv.page_stride * 2;
+    auto ask = [&](int j) {  // the entry, to be waited for
+        return s.table[min(j + 16 * (lane & 3), end - 1) >> a.kv.page_shift];
+    };
+    auto place = [&](int id, int j) {
+        const int jb = j + 16 * (lane & 3);
+        Pages t;
+        const bool there = (jb < end) & ((unsigned)id < (unsigned)a.kv.num_pages);
+        t.id = there ? id : -1;
+        t.off = (unsigned long long)(unsigned)max(t.id, 0) * page_bytes + (bytes_in + ((unsigned)jb & slots)) * ROW;
+        return t;
+    };
+    auto block_off = [&](const Pages& t, int b) {
+        return (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)t.off, b) |
+               (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(t.off >> 32), b) << 32;
+    };
+    // bit b: no page holds block b
+    auto holes_of = [&](const Pages& t) { return (unsigned)__ballot(t.id < 0) & 15u; };
+    auto fetch = [&](int buf, const Pages& t) {
         typedef __attribute__((address_space(3))) void* LP;
         typedef const __attribute__((address_space(1))) void* GP;
 #pragma unroll
         for (int n = 0; n < CI; n++) {
-            const int row = (4 * n + w) * WROWS;
-            const char* src = from + slot_off(a, page_of(pg, n), g, j + (row & ~15), D) * 2;
-            __builtin_amdgcn_global_load_lds((GP)(src + lane_src), (LP)(to + (4 * n + w) * 1024), 16, 0, 0);
+            const unsigned long long off = block_off(t, ROW == 256 ? n : 2 * n + (w >> 1));
+            char* to = sm + buf * TB + (4 * n + w) * 1024;
+            __builtin_amdgcn_global_load_lds((GP)(klane + off), (LP)to, 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((GP)(vlane + off), (LP)(to + 2 * TB), 16, 0, 0);
         }
-    };
-    auto pages_of = [&](int j, int (&pg)[BLOCKS]) {
-#pragma unroll
-        for (int b = 0; b < BLOCKS; b++) pg[b] = page_at(a, s, j + 16 * b, end);
     };
     // Values of rows that no row sees become zeros, and so does what is not
     // finite where some row must not meet it (three terms: anywhere); each
     // lane looks after the chunks it has loaded.
     const int least = s.sees(wk.row0 / a.group);
-    auto mend = [&](char* V, const int (&pg)[BLOCKS], int j) {
-        bool hole = false;
-#pragma unroll
-        for (int b = 0; b < BLOCKS; b++) hole |= pg[b] < 0;
-        const bool part = hole || j + N > least;
+    auto mend = [&](char* V, unsigned holes, int j) {
+        const bool part = holes || j + N > least;
         if (!part && TERMS == 1) return;
         uint32_t bits = 0;
         v4u v[CI];
 #pragma unroll
         for (int n = 0; n < CI; n++) {
+            const int row = (4 * n + w) * WROWS;
             v4u* at = (v4u*)(V + (4 * n + w) * 1024 + 16 * lane);
             v[n] = *at;
-            if (part && (page_of(pg, n) < 0 || j + (4 * n + w) * WROWS + lane_row >= end)) {
+            if (part && ((holes >> (row / 16) & 1) || j + row + lane_row >= end)) {
                 v[n] = v4u{0, 0, 0, 0};
                 *at = v[n];
             }
@@ -265,10 +284,9 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile_bf16(AttnArgs a) {
             for (int n = 0; n < CI; n++) *(v4u*)(V + (4 * n + w) * 1024 + 16 * lane) = finite_part<false>(v[n]);
         }
     };
-    // Scores of a tile, K's operands two steps ahead; beside(c): other work
-    // that goes between the products of step c, which keep the order written
-    // (left alone, the compiler loads all operands first and spills).
-    auto scores = [&](int K, v16f (&sc)[SB], auto beside) {
+    // Scores of a tile, K's operands two steps ahead (left alone, the compiler
+    // loads all of them first, and spills).
+    auto scores = [&](int K, v16f (&sc)[SB]) {
         // lds_slot(32 b + r, 2 c + p) = (lds_slot(r, p) ^ 32 c) + 32 b ROW, from
         // one register (hoisted out of the loop the places take eight)
         int at = K + lds_slot<ROW>(r, p);
@@ -292,49 +310,43 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile_bf16(AttnArgs a) {
 #pragma unroll
                 for (int b = 0; b < SB; b++)
                     sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ko[c % 3][b], __builtin_bit_cast(v8b, q[z][c]), sc[b], 0, 0, 0);
-            beside(c);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto nothing = [](int) {};
-
-    int pg[BLOCKS], p1[BLOCKS], p2[BLOCKS];  // pages of this tile and the next two
-    int j = beg;
+    int j = beg, ahead = 0;      // the table entry of the tile after next
+    unsigned holes = 0;
+    Pages next = {};
     if (j < end) {
-        pages_of(j, pg);
-        pages_of(j + N, p1);
-        pages_of(j + 2 * N, p2);
-        fetch(kc, sm, pg, j);
-        fetch(vc, sm + 2 * TB, pg, j);
-        if (AHEAD && j + N < end) fetch(kc, sm + TB, p1, j + N);
-#pragma unroll
-        for (int z = 0; z < TERMS; z++)
-#pragma unroll
-            for (int t = 0; t < KS; t++) arrived(q[z][t]);
+        const int e0 = ask(j), e1 = ask(j + N);
+        ahead = ask(j + 2 * N);
+        const Pages first = place(e0, j);
+        next = place(e1, j + N);
+        holes = holes_of(first);
+        fetch(0, first);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();  // odd_lo, odd_hi are set up
-        mend(sm + 2 * TB, pg, j);
+        mend(sm + 2 * TB, holes, j);
         __syncthreads();
     }
-    v16f sc[SB];
-    if (AHEAD && j < end && j < me.most) scores(0, sc, nothing);
-    for (int k = 0; j < end; k++, j += N) {
-        const int buf = k & 1, jn = j + N;
-        if (AHEAD) {
-            if (jn + N < end) fetch(kc, sm + buf * TB, p2, jn + N);
-            if (jn < end) fetch(vc, sm + (2 + (buf ^ 1)) * TB, p1, jn);
-        } else if (jn < end) {
-            fetch(kc, sm + (buf ^ 1) * TB, p1, jn);
-            fetch(vc, sm + (2 + (buf ^ 1)) * TB, p1, jn);
-        }
-        int p3[BLOCKS];
-        pages_of(jn + 2 * N, p3);
-        if (j < me.most) {
-            if (!AHEAD) scores(buf * TB, sc, nothing);
-            bool hole = false;
 #pragma unroll
-            for (int b = 0; b < BLOCKS; b++) hole |= pg[b] < 0;
-            const bool masked = hole || j + N > me.least || !me.whole;
+    for (int z = 0; z < TERMS; z++)
+#pragma unroll
+        for (int t = 0; t < KS; t++) arrived(q[z][t]);
+    float mu = -FLT_MAX;
+    bool far = false;
+    for (int buf = 0; j < end; buf ^= 1, j += N) {
+        const int jn = j + N;
+        unsigned next_holes = 0;
+        if (jn < end) {
+            next_holes = holes_of(next);
+            fetch(buf ^ 1, next);
+            next = place(ahead, jn + N);
+            ahead = ask(jn + 2 * N);
+        }
+        if (j < me.most) {
+            v16f sc[SB];
+            scores(buf * TB, sc);
+            const bool masked = holes || j + N > me.least || !me.whole;
             // element e of block b: position 32 b + 8 (e / 4) + 4 p + e % 4
             float mx = -FLT_MAX;
             if (masked) {
@@ -343,7 +355,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile_bf16(AttnArgs a) {
                 for (int b = 0; b < SB; b++)
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        const bool seen = pg[2 * b + e / 8] >= 0 && j + 32 * b + 8 * (e / 4) + 4 * p + e % 4 < me.sees;
+                        const bool seen = !(holes >> (2 * b + e / 8) & 1) && j + 32 * b + 8 * (e / 4) + 4 * p + e % 4 < me.sees;
                         sc[b][e] = seen ? sc[b][e] : -__builtin_huge_valf();
                         mx = seen ? -FLT_MAX : mx;
                     }
@@ -362,7 +374,7 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile_bf16(AttnArgs a) {
                         for (int e = 0; e < 16; e++)
                             if (sc[b][e] != sc[b][e]) {
                                 const float* qp = (const float*)a.q + qat;
-                                const uint16_t* kp = (const uint16_t*)kc + slot_off(a, pg[2 * b + e / 8], g, j + 32 * b + 16 * (e / 8), D) +
+                                const uint16_t* kp = (const uint16_t*)kc + slot_off(a, page_at(a, s, j + 32 * b + 16 * (e / 8), end), g, j + 32 * b + 16 * (e / 8), D) +
                                                      (8 * (e / 4 % 2) + 4 * p + e % 4) * D;
                                 float t = 0.0f;
                                 for (int d = 0; d < D; d++) t = fmaf(qp[d], __uint_as_float((uint32_t)kp[d] << 16), t);
@@ -380,33 +392,30 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile_bf16(AttnArgs a) {
                 mx = fmaxf(mx, y * a.c);
             }
             mx = fmaxf(mx, lane_xor<32>(mx));
+            float al = 1.0f;
             if (__any(mx > m + LAG)) {
-                const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - fmaxf(mn, -FLT_MAX));
-                l *= al;
-#pragma unroll
-                for (int t = 0; t < DT; t++) acc[t] *= al;
+                const float mn = fmaxf(m, mx);
+                mu = fmaxf(mn, -FLT_MAX);
+                al = __builtin_amdgcn_exp2f(m - mu);
                 m = mn;
+                far = __any(far_score(mu));
             }
-            float mu = fmaxf(m, -FLT_MAX), c = a.c;
-            if (__any(far_score(mu))) {
+            // (on every tile: behind a branch around it, the compiler keeps the
+            // sums in two sets of registers and copies them)
+            l *= al;
+#pragma unroll
+            for (int t = 0; t < DT; t++) acc[t] *= al;
+            if (far) {
 #pragma unroll
                 for (int b = 0; b < SB; b++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) sc[b][e] = sc[b][e] * c - mu;
-                c = 1.0f, mu = 0.0f;
-            }
-            // probabilities e0 .. e0 + n - 1 of the tile's 32, in place
-            auto probabilities = [&](int e0, int n) {
+                    for (int e = 0; e < 16; e++) sc[b][e] = __builtin_amdgcn_exp2f(sc[b][e] * a.c - mu);
+            } else {
 #pragma unroll
-                for (int e = e0; e < e0 + n; e++) {
-                    const float y = __builtin_amdgcn_exp2f(fmaf(sc[e / 16][e % 16], c, -mu));
-                    sc[e / 16][e % 16] = y;
-                    l += y;
-                }
-            };
-            v16f nx[SB];
-            if (AHEAD && jn < end && jn < me.most) scores((buf ^ 1) * TB, nx, [&](int step) { probabilities(step * (32 / KS), 32 / KS); });
-            else probabilities(0, 32);
+                for (int b = 0; b < SB; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) sc[b][e] = __builtin_amdgcn_exp2f(fmaf(sc[b][e], a.c, -mu));
+            }
             // lds_slot(16 ks + 8 h + row, ch + 4 t) = (lds_slot(row, ch) ^ 64 t ^ 32 h) + (16 ks + 8 h) ROW
             int vat = (2 + buf) * TB + lds_slot<ROW>(4 * p + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 8 * (lane & 1);
             asm volatile("" : "+v"(vat));
@@ -425,8 +434,11 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile_bf16(AttnArgs a) {
                 for (int e = 0; e < 4; e++) {
                     const float y0 = sc[ks / 2][8 * (ks % 2) + 2 * e], y1 = sc[ks / 2][8 * (ks % 2) + 2 * e + 1];
                     if constexpr (TERMS == 1) {
+                        // (l sums what the values are weighted with)
                         pb[0][e] = pack_bf16(y0, y1);
+                        l = add_bf16(pb[0][e], l);
                     } else {
+                        l += y0 + y1;
                         float t0[3], t1[3];
                         three_terms(y0, t0);
                         three_terms(y1, t1);
@@ -444,16 +456,11 @@ __global__ __launch_bounds__(THREADS, 2) void k_tile_bf16(AttnArgs a) {
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            if (AHEAD) {
-#pragma unroll
-                for (int b = 0; b < SB; b++) sc[b] = nx[b];
-            }
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the fetches)
-        if (jn < end) mend(sm + (2 + (buf ^ 1)) * TB, p1, jn);
+        if (jn < end) mend(sm + (2 + (buf ^ 1)) * TB, next_holes, jn);
         __syncthreads();
-#pragma unroll
-        for (int b = 0; b < BLOCKS; b++) pg[b] = p1[b], p1[b] = p2[b], p2[b] = p3[b];
+        holes = next_holes;
     }
     __syncthreads();
     if (odd_hi) meet_odd_tile<typename std::conditional<F32Q, float, uint16_t>::type, uint16_t, D>(a, wk, me, qat, odd_lo, odd_hi, m, [&](int t, int e) { return 32 * t + 8 * (e / 4) + 4 * p + e % 4; }, acc);
