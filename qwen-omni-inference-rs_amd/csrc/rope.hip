@@ -8,11 +8,11 @@
 // of a turn and handed to the float32 Taylor sums of sin and cos (the next
 // terms are below 3e-8 at pi / 4).
 //
-// A thread has 2 V elements of a head: V consecutive pairs, V = 16 bytes of
-// elements, or V from each half of what passes through.  head_dim / (2 V)
-// threads make a head, and a workgroup's threads go over the heads of one row
-// in steps that keep their pairs where that divides, so that the sines are
-// computed once a thread.
+// A workgroup takes a few rows: its threads compute the sines of the rows'
+// pairs into LDS, once for all heads, and go over the heads.  A thread has 2 V
+// elements of a head: V consecutive pairs, V = 16 bytes of elements, or 2 V of
+// what passes through; head_dim / (2 V) threads make a head.
+#include <algorithm>
 #include <cmath>
 #include <new>
 
@@ -103,27 +103,34 @@ struct Unit {
     }
 };
 
-template <int V>
-__device__ __forceinline__ void angles(const RopePair* table, int p0, const int32_t* positions, size_t stride, int row,
-                                       int fallback, bool inverse, float (&c)[V], float (&s)[V]) {
-#pragma unroll
-    for (int i = 0; i < V; i++) {
-        const RopePair p = table[p0 + i];
-        const int at = positions ? positions[p.axis * stride + row] : fallback;
-        turn(at, p.turns, &c[i], &s[i]);
-        if (inverse) s[i] = -s[i];
+// cos and sin of `rows` rows from row0 on into sc [row][half], by the whole
+// workgroup; at(i, axis): position of row row0 + i.
+template <typename F>
+__device__ __forceinline__ void sines(const RopePair* table, int half, int rows, float2* sc, F at) {
+    for (int x = threadIdx.x; x < rows * half; x += RT) {
+        const int i = x / half;
+        const RopePair p = table[x - i * half];
+        float2 v;
+        turn(at(i, p.axis), p.turns, &v.x, &v.y);
+        sc[x] = v;
     }
 }
 
 template <int V>
-__device__ __forceinline__ void rotate(float (&a)[V], float (&b)[V], const float (&c)[V], const float (&s)[V]) {
+__device__ __forceinline__ void rotate(float (&a)[V], float (&b)[V], const float2* sc, float sign) {
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        const float x = a[i], y = b[i];
-        a[i] = fmaf(x, c[i], -(y * s[i]));
-        b[i] = fmaf(y, c[i], x * s[i]);
+    for (int i = 0; i < V; i += 2) {
+        const float4 s = *(const float4*)(sc + i);
+        const float s0 = s.y * sign, s1 = s.w * sign;
+        const float x0 = a[i], y0 = b[i], x1 = a[i + 1], y1 = b[i + 1];
+        a[i] = fmaf(x0, s.x, -(y0 * s0));
+        b[i] = fmaf(y0, s.x, x0 * s0);
+        a[i + 1] = fmaf(x1, s.z, -(y1 * s1));
+        b[i + 1] = fmaf(y1, s.z, x1 * s1);
     }
 }
+
+constexpr int ROWS_MAX = 8;  // rows of a workgroup
 
 struct RopeArgs {
     const RopePair* table;
@@ -132,30 +139,28 @@ struct RopeArgs {
     size_t xs, ys;  // bytes
     const int32_t* positions;
     size_t ps;
-    int rows, heads, half, units, dim;
-    bool inverse;
+    int rows, heads, half, units, dim, per;  // per: rows of a workgroup
+    float sign;
 };
 
 template <typename T>
 __global__ __launch_bounds__(RT) void k_rope(RopeArgs a) {
     constexpr int V = Vec<T>::V;
-    const int row = blockIdx.x, total = a.heads * a.units, step = gridDim.y * RT;
-    float c[V], s[V];
-    int have = -1;
-    for (int item = blockIdx.y * RT + threadIdx.x; item < total; item += step) {
-        const int h = item / a.units, u = item - h * a.units;
+    __shared__ __attribute__((aligned(16))) float2 sc[ROWS_MAX * 128];
+    const int row0 = blockIdx.x * a.per, rows = min(a.per, a.rows - row0);
+    sines(a.table, a.half, rows, sc, [&](int i, int axis) { return a.positions[axis * a.ps + row0 + i]; });
+    __syncthreads();
+    const int each = a.heads * a.units, total = rows * each;
+    for (int item = blockIdx.y * RT + threadIdx.x; item < total; item += gridDim.y * RT) {
+        const int i = item / each, in = item - i * each, h = in / a.units, u = in - h * a.units;
         const Unit<V> w(u, a.half);
         const size_t off = (size_t)h * a.dim * sizeof(T);
-        const char* x = a.x + row * a.xs + off;
-        char* y = a.y + row * a.ys + off;
+        const char* x = a.x + (row0 + i) * a.xs + off;
+        char* y = a.y + (row0 + i) * a.ys + off;
         float p[V], q[V];
         Vec<T>::load(x + w.lo * sizeof(T), p);
         Vec<T>::load(x + w.hi * sizeof(T), q);
-        if (w.turns) {
-            if (u != have) angles<V>(a.table, u * V, a.positions, a.ps, row, 0, a.inverse, c, s);
-            have = u;
-            rotate<V>(p, q, c, s);
-        }
+        if (w.turns) rotate<V>(p, q, sc + i * a.half + u * V, a.sign);
         Vec<T>::store(y + w.lo * sizeof(T), p);
         Vec<T>::store(y + w.hi * sizeof(T), q);
     }
@@ -172,26 +177,36 @@ struct AppendArgs {
     float eps;
     const int32_t* positions;
     size_t ps;
-    int heads, half;
+    int heads, half, per;  // per: rows of a workgroup
 };
 
-// The sequence of a row, by all threads of the workgroup; -1: none.
-__device__ __forceinline__ int sequence_of(const BatchDev& b, int row, int* first, int* total) {
+// Where a row goes: its position in its sequence, and the page and slot of it
+// (page -1: none); seq < 0: no sequence has the row.
+struct Place {
+    int seq, slot, page;
+};
+
+// The places of `rows` rows from row0 on, by the whole workgroup.
+__device__ __forceinline__ void find_places(const AppendArgs& a, int row0, int rows, Place* places) {
+    const BatchDev& b = a.batch;
+    if ((int)threadIdx.x < rows) places[threadIdx.x] = {-1, 0, -1};
+    __syncthreads();
+    auto put = [&](int i, int s, const RowRange& r) {
+        const int64_t slot = (int64_t)b.lengths[s] - r.total + (row0 + i - r.first);
+        int page = -1;
+        if (slot >= 0 && slot < (int64_t)b.max_pages << a.kv.page_shift) page = b.pages[(size_t)s * b.max_pages + (slot >> a.kv.page_shift)];
+        places[i] = {s, (int)slot, (unsigned)page < (unsigned)a.kv.num_pages ? page : -1};
+    };
     if (!b.row_begin) {
-        *first = row, *total = 1;
-        return row;
-    }
-    __shared__ int found[3];
-    if (threadIdx.x == 0) found[0] = -1;
-    __syncthreads();
-    for (int s = threadIdx.x; s < b.batch; s += RT) {
-        const RowRange r = rows_of(b, s);
-        // at most one sequence of an ascending row_begin has the row
-        if (row >= r.first && row - r.first < r.count) found[0] = s, found[1] = r.first, found[2] = r.total;
+        if ((int)threadIdx.x < rows) put(threadIdx.x, row0 + threadIdx.x, {row0 + (int)threadIdx.x, 1, 1});
+    } else {
+        for (int s = threadIdx.x; s < b.batch; s += RT) {
+            const RowRange r = rows_of(b, s);
+            // (an ascending row_begin gives a row one sequence at most)
+            for (int i = max(0, r.first - row0); i < min(rows, r.first + r.count - row0); i++) put(i, s, r);
+        }
     }
     __syncthreads();
-    *first = found[1], *total = found[2];
-    return found[0];
 }
 
 // x * rsqrt(mean(x^2) + eps) * w of a head whose LANES threads lie side by
@@ -212,35 +227,35 @@ __device__ __forceinline__ void norm_head(float (&a)[V], float (&b)[V], const fl
     const double inv = 1.0 / sqrt(sum / (double)(2 * V * LANES) + (double)eps);
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        a[i] = (float)(__bf16)(float)((double)a[i] * inv * (double)(float)(__bf16)w[u.lo + i]);
-        b[i] = (float)(__bf16)(float)((double)b[i] * inv * (double)(float)(__bf16)w[u.hi + i]);
+        // (a product of two bf16 is exact in float32)
+        a[i] = (float)(__bf16)(float)((double)(a[i] * (float)(__bf16)w[u.lo + i]) * inv);
+        b[i] = (float)(__bf16)(float)((double)(b[i] * (float)(__bf16)w[u.hi + i]) * inv);
     }
 }
 
-// One row of the batch: its q heads to q_out, its k and v heads to its slot.
+// Rows of the batch: their q heads to q_out, their k and v heads to their slots.
 template <typename T, typename C, int D>
 __global__ __launch_bounds__(RT) void k_append(AppendArgs a) {
     constexpr int V = Vec<T>::V, UNITS = D / (2 * V);
     static_assert(RT % UNITS == 0 && 64 % UNITS == 0, "a head's threads lie in one wave");
-    const int row = blockIdx.x;
-    int first, total_rows;
-    const int seq = sequence_of(a.batch, row, &first, &total_rows);
-    if (seq < 0) return;  // no sequence has the row
-    const int64_t slot = (int64_t)a.batch.lengths[seq] - total_rows + (row - first);
-    int page = -1;
-    if (slot >= 0 && slot < (int64_t)a.batch.max_pages << a.kv.page_shift)
-        page = a.batch.pages[(size_t)seq * a.batch.max_pages + (slot >> a.kv.page_shift)];
-    if (page >= a.kv.num_pages) page = -1;
-    const int in_page = (int)slot & ((1 << a.kv.page_shift) - 1);
-    const int qh = a.q ? a.heads : 0, total = (qh + 2 * a.kv.kv_heads) * UNITS;
+    __shared__ __attribute__((aligned(16))) float2 sc[ROWS_MAX * D / 2];
+    __shared__ Place places[ROWS_MAX];
+    const int row0 = blockIdx.x * a.per, rows = min(a.per, a.batch.rows - row0);
+    find_places(a, row0, rows, places);
+    if (a.table) {
+        sines(a.table, a.half, rows, sc, [&](int i, int axis) { return a.positions ? a.positions[axis * a.ps + row0 + i] : places[i].slot; });
+        __syncthreads();
+    }
+    const int qh = a.q ? a.heads : 0, each = qh + 2 * a.kv.kv_heads;
     const int u = threadIdx.x % UNITS;
     const Unit<V> w(u, a.half);
-    float c[V], s[V];
-    if (a.table && w.turns) angles<V>(a.table, u * V, a.positions, a.ps, row, (int)slot, false, c, s);
-    for (int item = blockIdx.y * RT + threadIdx.x; item < total; item += gridDim.y * RT) {
-        const int h = item / UNITS;  // whole heads: RT is a multiple of UNITS, so is total
+    const int step = gridDim.y * (RT / UNITS);
+    for (int item = blockIdx.y * (RT / UNITS) + threadIdx.x / UNITS; item < rows * each; item += step) {
+        const int i = item / each, h = item - i * each, row = row0 + i;
+        const Place at = places[i];
         const bool isq = h < qh, isk = !isq && h < qh + a.kv.kv_heads;
         const int g = isq ? h : isk ? h - qh : h - qh - a.kv.kv_heads;
+        if (at.seq < 0 || (!isq && at.page < 0)) continue;
         const char* src = (isq ? a.q + row * a.qs : isk ? a.k + row * a.ks : a.v + row * a.vs) + (size_t)g * D * sizeof(T);
         float p[V], q[V];
         Vec<T>::load(src + w.lo * sizeof(T), p);
@@ -248,24 +263,32 @@ __global__ __launch_bounds__(RT) void k_append(AppendArgs a) {
         if (isq || isk) {
             const float* nw = isq ? a.q_norm : a.k_norm;
             if (nw) norm_head<UNITS, V>(p, q, nw, w, a.eps);
-            if (a.table && w.turns) rotate<V>(p, q, c, s);
+            if (a.table && w.turns) rotate<V>(p, q, sc + i * a.half + u * V, 1.0f);
         }
         if (isq) {
             char* y = a.q_out + row * a.qos + (size_t)g * D * sizeof(T);
             Vec<T>::store(y + w.lo * sizeof(T), p);
             Vec<T>::store(y + w.hi * sizeof(T), q);
-        } else if (page >= 0) {
-            C* y = (C*)(isk ? a.kv.k : a.kv.v) + page * a.kv.page_stride + (((size_t)g << a.kv.page_shift) + in_page) * D;
+        } else {
+            const int in = at.slot & ((1 << a.kv.page_shift) - 1);
+            C* y = (C*)(isk ? a.kv.k : a.kv.v) + at.page * a.kv.page_stride + (((size_t)g << a.kv.page_shift) + in) * D;
             store_cache<C, V>(y + w.lo, p);
             store_cache<C, V>(y + w.hi, q);
         }
     }
 }
 
-// Workgroups that share a row's heads: so many that about two a CU run.
-unsigned head_parts(size_t rows, size_t items, int cus) {
-    const size_t most = (items + RT - 1) / RT, want = (2 * (size_t)cus + rows - 1) / rows;
-    return (unsigned)(want < most ? want : most);
+// Rows of a workgroup and workgroups that share them: few rows leave a
+// workgroup each, and their heads to several, so that two a CU run; many are
+// taken up to eight at a time while eight workgroups a CU are left.
+struct RowSplit {
+    int per;
+    dim3 grid;
+};
+RowSplit split_rows(size_t rows, size_t items, int cus) {
+    const size_t per = std::max<size_t>(1, std::min<size_t>(ROWS_MAX, rows / (8 * (size_t)cus)));
+    const size_t groups = (rows + per - 1) / per, most = (per * items + RT - 1) / RT, want = (2 * (size_t)cus + groups - 1) / groups;
+    return {(int)per, dim3((unsigned)groups, (unsigned)std::min(want, most))};
 }
 
 template <typename T, typename C>
@@ -468,11 +491,12 @@ lq8_status lq8_rope_device(lq8_ctx* ctx, const lq8_rope* rope, const lq8_rope_ro
     const bool f32 = rows->dtype == LQ8_DTYPE_F32;
     const int units = (int)rope->cfg.head_dim / (2 * (f32 ? 4 : 8));
     RopeArgs a{(const RopePair*)rope->table, (const char*)rows->x, (char*)rows->y, xs * es, ys * es, rows->positions, ps,
-               (int)rows->rows, (int)rows->heads, (int)rope->cfg.rotary_dim / 2, units, (int)rope->cfg.head_dim,
-               rows->inverse != 0};
-    const dim3 grid(rows->rows, head_parts(rows->rows, (size_t)rows->heads * units, ctx->num_cus));
-    if (f32) hipLaunchKernelGGL(k_rope<float>, grid, dim3(RT), 0, ctx->stream, a);
-    else hipLaunchKernelGGL(k_rope<Bf16>, grid, dim3(RT), 0, ctx->stream, a);
+               (int)rows->rows, (int)rows->heads, (int)rope->cfg.rotary_dim / 2, units, (int)rope->cfg.head_dim, 1,
+               rows->inverse ? -1.0f : 1.0f};
+    const RowSplit r = split_rows(rows->rows, (size_t)rows->heads * units, ctx->num_cus);
+    a.per = r.per;
+    if (f32) hipLaunchKernelGGL(k_rope<float>, r.grid, dim3(RT), 0, ctx->stream, a);
+    else hipLaunchKernelGGL(k_rope<Bf16>, r.grid, dim3(RT), 0, ctx->stream, a);
     LQ8_HIP(hipGetLastError());
     return LQ8_OK;
 }
@@ -518,10 +542,11 @@ lq8_status lq8_paged_append_device(lq8_ctx* ctx, const lq8_rope* rope, const lq8
     a.positions = rows->positions, a.ps = ps;
     a.heads = rows->q ? (int)rows->num_heads : 0;
     const size_t units = d / (2 * (rows->dtype == LQ8_DTYPE_F32 ? 4 : 8));
-    const dim3 grid(batch->rows, head_parts(batch->rows, (a.heads + 2 * (size_t)kv->num_kv_heads) * units, ctx->num_cus));
-    if (types == PT_F32_F32) launch_append<float, float>(a, grid, (int)d, ctx->stream);
-    else if (types == PT_F32_BF16) launch_append<float, Bf16>(a, grid, (int)d, ctx->stream);
-    else launch_append<Bf16, Bf16>(a, grid, (int)d, ctx->stream);
+    const RowSplit r = split_rows(batch->rows, (a.heads + 2 * (size_t)kv->num_kv_heads) * units, ctx->num_cus);
+    a.per = r.per;
+    if (types == PT_F32_F32) launch_append<float, float>(a, r.grid, (int)d, ctx->stream);
+    else if (types == PT_F32_BF16) launch_append<float, Bf16>(a, r.grid, (int)d, ctx->stream);
+    else launch_append<Bf16, Bf16>(a, r.grid, (int)d, ctx->stream);
     LQ8_HIP(hipGetLastError());
     return LQ8_OK;
 }
