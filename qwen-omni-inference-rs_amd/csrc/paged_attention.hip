@@ -129,12 +129,10 @@ lq8_status launch_join(const AttnArgs& a, bool f32, int dim, size_t slots, hipSt
     return LQ8_OK;
 }
 
-// How a call runs: which kernel takes each part, and its cuts.
+// How a call runs.
 struct Plan {
-    bool own_few = false, pre_few = false;
-    int own_blocks = 1, pre_blocks = 1;
-    size_t own_tiles = 0, pre_tiles = 0;  // row tiles over all spans, at most
-    size_t slots = 0, scratch = 0;        // of partial results; their bytes
+    size_t own_blocks = 0, pre_blocks = 0;  // workgroups of each part
+    size_t slots = 0, scratch = 0;          // of partial results; their bytes
 };
 
 constexpr int FEW_FILL = 8, TILE_FILL = 2;
@@ -160,22 +158,28 @@ Cut cut_of(size_t most, size_t groups, int cus, bool few, bool f32_pages) {
     return c;
 }
 
+// Row tiles of 16 read the cache once each (from the XCD's L2 behind the
+// first), tiles of 128 once for all, with a workgroup's waves on rows of
+// their own: up to FEW_MOST packed rows the first.
+constexpr size_t FEW_MOST = 64;
+
 Plan plan_of(AttnArgs* a, PagedTypes types, int dim, int cus) {
     Plan p;
     const size_t G = a->group, kvh = a->kv.kv_heads, rows = a->batch.rows, batch = a->batch.batch;
     const bool f32 = types == PT_F32_F32;
-    const size_t own = (size_t)a->batch.max_rows * G, each = (own + TILE_PACKED - 1) / TILE_PACKED;
-    p.own_few = own <= FEW_MAX_ROWS;
-    p.own_blocks = own <= 16 ? 1 : 2;
-    p.own_tiles = p.own_few ? batch : std::min(batch * each, (rows * G + (TILE_PACKED - 1) * std::min(batch, rows)) / TILE_PACKED);
-    a->own = cut_of((size_t)a->batch.max_pages << a->kv.page_shift, p.own_tiles * kvh, cus, p.own_few, f32);
+    // row tiles of `spans` spans that have `all` rows together and at most `most` each
+    auto part = [&](size_t spans, size_t all, size_t most, uint32_t pages, Cut* cut, int* few) {
+        const size_t packed = most * G;
+        *few = packed <= FEW_MOST ? (int)((packed + FEW_PACKED - 1) / FEW_PACKED) : 0;
+        const size_t each = (packed + TILE_PACKED - 1) / TILE_PACKED, held = std::min(spans, all);
+        const size_t tiles = *few ? spans * *few : std::min(spans * each, (all * G + (TILE_PACKED - 1) * held) / TILE_PACKED);
+        *cut = cut_of((size_t)pages << a->kv.page_shift, tiles * kvh, cus, *few > 0, f32);
+        return tiles * kvh * cut->pieces;
+    };
+    p.own_blocks = part(batch, rows, a->batch.max_rows, a->batch.max_pages, &a->own, &a->own_few);
     p.slots = a->own.pieces;
     if (a->prefix.groups) {
-        const size_t groups = a->prefix.groups;
-        p.pre_few = rows * G <= FEW_MAX_ROWS;
-        p.pre_blocks = rows * G <= 16 ? 1 : 2;
-        p.pre_tiles = p.pre_few ? groups : (rows * G + (TILE_PACKED - 1) * std::min(groups, rows)) / TILE_PACKED;
-        a->pre = cut_of((size_t)a->prefix.max_pages << a->kv.page_shift, p.pre_tiles * kvh, cus, p.pre_few, f32);
+        p.pre_blocks = part(a->prefix.groups, rows, rows, a->prefix.max_pages, &a->pre, &a->pre_few);
         p.slots += a->pre.pieces;
     }
     if (p.slots > 1) p.scratch = p.slots * rows * a->heads * (dim * sizeof(float) + sizeof(float2));
@@ -218,8 +222,8 @@ lq8_status check_attention(const lq8_kv_pages* kv, const lq8_paged_batch* batch,
     a->c = rows->scale * 1.4426950408889634f;
     if (batch->batch == 0 || batch->rows == 0) return LQ8_OK;
     const Plan p = plan_of(a, *types, (int)kv->head_dim, 1);
-    if (std::max(p.own_tiles, p.pre_tiles) * kv->num_kv_heads >= ((size_t)1 << 32) / 256)
-        return fail(LQ8_ERR_SHAPE_MISMATCH, "attention: sequences times kv heads above 2^24");
+    if (p.own_blocks + p.pre_blocks >= ((size_t)1 << 32) / 256 / 2)
+        return fail(LQ8_ERR_SHAPE_MISMATCH, "attention: sequences times kv heads above 2^23");
     return LQ8_OK;
 }
 
@@ -241,11 +245,13 @@ lq8_status attention(lq8_ctx* ctx, const lq8_kv_pages* kv, const lq8_paged_batch
         a.part = (float*)sc;
         a.ml = (float2*)(a.part + p.slots * batch->rows * a.heads * dim);
     }
-    if (a.prefix.groups) {
-        st = p.pre_few ? launch_few(ctx->stream, a, types, dim, p.pre_blocks, true) : launch_tile(ctx->stream, a, types, dim, p.pre_tiles, true);
-        if (st) return st;
+    if (a.prefix.groups && a.own_few) {
+        st = launch_both(ctx->stream, a, types, dim, p.pre_blocks, p.own_blocks, a.pre_few == 0);
+    } else {
+        // (a prefix's rows are at least one sequence's)
+        if (a.prefix.groups) st = launch_tile(ctx->stream, a, types, dim, p.pre_blocks, true);
+        if (!st) st = a.own_few ? launch_few(ctx->stream, a, types, dim, p.own_blocks, false) : launch_tile(ctx->stream, a, types, dim, p.own_blocks, false);
     }
-    st = p.own_few ? launch_few(ctx->stream, a, types, dim, p.own_blocks, false) : launch_tile(ctx->stream, a, types, dim, p.own_tiles, false);
     if (st || p.slots == 1) return st;
     return launch_join(a, rows->dtype == LQ8_DTYPE_F32, dim, p.slots, ctx->stream);
 }
@@ -277,15 +283,14 @@ lq8_status lq8_paged_plan(const lq8_kv_pages* kv, const lq8_paged_batch* batch, 
     *out = {};
     if (batch->batch == 0 || batch->rows == 0) return LQ8_OK;
     const Plan p = plan_of(&a, types, (int)kv->head_dim, (int)num_workgroups);
-    out->own_rows = p.own_few ? 16 * p.own_blocks : TILE_PACKED;
+    out->own_rows = a.own_few ? FEW_PACKED : TILE_PACKED;
     out->own_splits = a.own.pieces;
     out->own_chunk = a.own.shortest;
-    out->workgroups = p.own_tiles * kv->num_kv_heads * a.own.pieces;
+    out->workgroups = p.own_blocks + p.pre_blocks;
     if (a.prefix.groups) {
-        out->prefix_rows = p.pre_few ? 16 * p.pre_blocks : TILE_PACKED;
+        out->prefix_rows = a.pre_few ? FEW_PACKED : TILE_PACKED;
         out->prefix_splits = a.pre.pieces;
         out->prefix_chunk = a.pre.shortest;
-        out->workgroups += p.pre_tiles * kv->num_kv_heads * a.pre.pieces;
     }
     out->scratch_bytes = p.scratch;
     return LQ8_OK;

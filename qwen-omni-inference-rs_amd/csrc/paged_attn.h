@@ -1,5 +1,5 @@
 // paged_attn.h -- what the kernels of attention over a paged cache share
-// (paged_few.hip, paged_tile.hip, paged_attention.hip).
+// (paged_few.h, paged_tile.h, paged_attention.hip).
 //
 // Rows.  The queries of a kv head are packed: packed row r of a sequence (or
 // of a group's rows) is query head r % G of row r / G, G = num_heads /
@@ -43,6 +43,7 @@ struct AttnArgs {
     int heads, group;
     float c;        // scale * log2(e)
     Cut own, pre;
+    int own_few = 0, pre_few = 0;  // row tiles of a span in launch_few's kernel (0: launch_tile's)
     float* part;    // [slots][rows][heads][head_dim], own pieces first; null: one piece, results go to out
     float2* ml;     // [slots][rows][heads]
 };
@@ -203,9 +204,12 @@ __device__ __forceinline__ void meet_odd(const AttnArgs& a, const Span& s, int g
         }
 }
 
-lq8_status launch_few(hipStream_t s, const AttnArgs& a, PagedTypes types, int dim, int blocks, bool prefix);
-constexpr int FEW_MAX_ROWS = 32;  // packed rows launch_few takes
-lq8_status launch_tile(hipStream_t s, const AttnArgs& a, PagedTypes types, int dim, size_t tiles, bool prefix);
-constexpr int TILE_PACKED = 128;  // packed rows of a launch_tile workgroup
+constexpr int FEW_PACKED = 16;    // packed rows of a launch_few block
+constexpr int TILE_PACKED = 128;  // of a launch_tile one
+// `blocks` workgroups of the prefix part or of the own one; launch_both: of
+// both, the prefix by launch_tile's kernel or launch_few's, the own by launch_few's.
+lq8_status launch_few(hipStream_t s, const AttnArgs& a, PagedTypes types, int dim, size_t blocks, bool prefix);
+lq8_status launch_tile(hipStream_t s, const AttnArgs& a, PagedTypes types, int dim, size_t blocks, bool prefix);
+lq8_status launch_both(hipStream_t s, const AttnArgs& a, PagedTypes types, int dim, size_t pre, size_t own, bool tile);
 
 }  // namespace lq8
