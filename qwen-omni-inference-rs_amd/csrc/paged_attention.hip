@@ -135,51 +135,74 @@ struct Plan {
     size_t slots = 0, scratch = 0;          // of partial results; their bytes
 };
 
-constexpr int FEW_FILL = 8, TILE_FILL = 2;
+// Workgroups a compute unit that a part is cut into.  Tiles beside own
+// positions (PRE_FILL) leave these half the machine, and fewer pieces are less
+// to join: 64 rows behind 8192 positions 64, 45, 45, 49 and 59 us at 0.25, 0.5,
+// 0.75, 1 and 2.  Tiles alone: a chunk of f32 243, 222 and 233 us at 1, 2 and 4.
+// Few rows: 206, 204 and 203 us at 4, 8 and 16 (64 sequences of bf16).
+constexpr float FEW_FILL = 8, TILE_FILL = 2, PRE_FILL = 0.5f;
+
+size_t few_unit(bool f32_pages) { return f32_pages ? 64 : 128; }  // a tile for each of the four waves
 
 // Pieces of a part whose positions are at most `most`, in `groups` workgroups
 // a piece.  few: its kernel takes spans one by one, so that a long one among
 // short ones needs pieces of its own.
-Cut cut_of(size_t most, size_t groups, int cus, bool few, bool f32_pages) {
+Cut cut_of(size_t most, size_t groups, int cus, bool few, bool f32_pages, float fill) {
     Cut c;
     size_t pieces;
     if (few) {
-        c.unit = f32_pages ? 64 : 128;  // a tile for each of the four waves
+        c.unit = few_unit(f32_pages);
         c.shortest = c.unit;
         const size_t longest = (most + 2047) / 2048, cap = 32768 / groups;
-        pieces = std::max((size_t)FEW_FILL * cus / groups, std::min(longest, cap));
+        pieces = std::max((size_t)(FEW_FILL * cus) / groups, std::min(longest, cap));
     } else {
         c.unit = f32_pages ? 32 : 64;
         c.shortest = 256;
-        pieces = (size_t)TILE_FILL * cus / groups;
+        pieces = (size_t)(fill * cus) / groups;
     }
     c.shift = __builtin_ctz(c.shortest);
     c.pieces = (int)std::max<size_t>(1, std::min(pieces, (most + c.shortest - 1) / c.shortest));
     return c;
 }
 
-// Row tiles of 16 read the cache once each (from the XCD's L2 behind the
-// first), tiles of 128 once for all, with a workgroup's waves on rows of
-// their own: up to FEW_MOST packed rows the first.
-constexpr size_t FEW_MOST = 64;
+// Row tiles of 16 fill their products but read the cache once each; tiles of
+// 128 read it once, with a workgroup's waves on 32 rows each (of few rows some
+// have none).  us, 16-row tiles / 128-row tiles, 32 heads over 8 of 128, 8 x
+// 4000 positions, by packed rows:
+//     packed                32            48            64            96
+//     bf16                  42 /  23      52 /  27      61 /  26      80 /  29
+//     f32 over bf16         42 /  37      47 /  45      57 /  45      69 /  48
+//     f32                   58 /  82      80 / 120      98 / 115     133 / 118
+// and 32 x 2000: f32 over bf16 55 / 64, 67 / 86, 82 / 86, 112 / 90.  Where the
+// blocks of 16 rows by a piece are at most two a compute unit, latency decides:
+// 1 x 2000 of bf16 11 / 15, 13 / 17, 14 / 16 and (three a unit) 18 / 18.
+bool takes_few(PagedTypes types, size_t packed, size_t blocks, int cus) {
+    return packed <= (types == PT_BF16_BF16 ? 16 : types == PT_F32_BF16 ? 48 : 64) || blocks <= 2 * (size_t)cus;
+}
 
 Plan plan_of(AttnArgs* a, PagedTypes types, int dim, int cus) {
     Plan p;
     const size_t G = a->group, kvh = a->kv.kv_heads, rows = a->batch.rows, batch = a->batch.batch;
     const bool f32 = types == PT_F32_F32;
-    // row tiles of `spans` spans that have `all` rows together and at most `most` each
-    auto part = [&](size_t spans, size_t all, size_t most, uint32_t pages, Cut* cut, int* few) {
-        const size_t packed = most * G;
-        *few = packed <= FEW_MOST ? (int)((packed + FEW_PACKED - 1) / FEW_PACKED) : 0;
-        const size_t each = (packed + TILE_PACKED - 1) / TILE_PACKED, held = std::min(spans, all);
-        const size_t tiles = *few ? spans * *few : std::min(spans * each, (all * G + (TILE_PACKED - 1) * held) / TILE_PACKED);
-        *cut = cut_of((size_t)pages << a->kv.page_shift, tiles * kvh, cus, *few > 0, f32);
+    // row tiles of `spans` spans that have `all` rows together, at most `most` each and `usual` by the rule's reckoning
+    auto part = [&](size_t spans, size_t all, size_t most, size_t usual, uint32_t pages, Cut* cut, int* few, bool* one, float fill) {
+        const size_t positions = (size_t)pages << a->kv.page_shift, units = (positions + few_unit(f32) - 1) / few_unit(f32);
+        auto tiles_of = [&](size_t rows) {
+            return std::min(spans * ((most * G + rows - 1) / rows), (all * G + (rows - 1) * std::min(spans, all)) / rows);
+        };
+        *one = most * G <= FEW_PACKED;
+        size_t tiles = *one ? spans : tiles_of(FEW_PACKED);
+        const bool is_few = takes_few(types, usual * G, tiles * kvh * units, cus);
+        *few = is_few ? (int)tiles : 0;
+        if (!is_few) tiles = tiles_of(TILE_PACKED);
+        *cut = cut_of(positions, tiles * kvh, cus, is_few, f32, fill);
         return tiles * kvh * cut->pieces;
     };
-    p.own_blocks = part(batch, rows, a->batch.max_rows, a->batch.max_pages, &a->own, &a->own_few);
+    p.own_blocks = part(batch, rows, a->batch.max_rows, a->batch.max_rows, a->batch.max_pages, &a->own, &a->own_few, &a->own_each, TILE_FILL);
     p.slots = a->own.pieces;
     if (a->prefix.groups) {
-        p.pre_blocks = part(a->prefix.groups, rows, rows, a->prefix.max_pages, &a->pre, &a->pre_few);
+        const size_t groups = a->prefix.groups;  // (each may have all rows)
+        p.pre_blocks = part(groups, rows, rows, (rows + groups - 1) / groups, a->prefix.max_pages, &a->pre, &a->pre_few, &a->pre_each, a->own_few ? PRE_FILL : TILE_FILL);
         p.slots += a->pre.pieces;
     }
     if (p.slots > 1) p.scratch = p.slots * rows * a->heads * (dim * sizeof(float) + sizeof(float2));
@@ -248,9 +271,8 @@ lq8_status attention(lq8_ctx* ctx, const lq8_kv_pages* kv, const lq8_paged_batch
     if (a.prefix.groups && a.own_few) {
         st = launch_both(ctx->stream, a, types, dim, p.pre_blocks, p.own_blocks, a.pre_few == 0);
     } else {
-        // (a prefix's rows are at least one sequence's)
-        if (a.prefix.groups) st = launch_tile(ctx->stream, a, types, dim, p.pre_blocks, true);
-        if (!st) st = a.own_few ? launch_few(ctx->stream, a, types, dim, p.own_blocks, false) : launch_tile(ctx->stream, a, types, dim, p.own_blocks, false);
+        if (a.prefix.groups) st = (a.pre_few ? launch_few : launch_tile)(ctx->stream, a, types, dim, p.pre_blocks, true);
+        if (!st) st = (a.own_few ? launch_few : launch_tile)(ctx->stream, a, types, dim, p.own_blocks, false);
     }
     if (st || p.slots == 1) return st;
     return launch_join(a, rows->dtype == LQ8_DTYPE_F32, dim, p.slots, ctx->stream);

@@ -43,7 +43,8 @@ struct AttnArgs {
     int heads, group;
     float c;        // scale * log2(e)
     Cut own, pre;
-    int own_few = 0, pre_few = 0;  // row tiles of a span in launch_few's kernel (0: launch_tile's)
+    int own_few = 0, pre_few = 0;  // row tiles, at most, in launch_few's kernel (0: launch_tile's)
+    bool own_each = false, pre_each = false;  // of these tile t is all rows of span t
     float* part;    // [slots][rows][heads][head_dim], own pieces first; null: one piece, results go to out
     float2* ml;     // [slots][rows][heads]
 };
@@ -76,6 +77,46 @@ __device__ __forceinline__ Span prefix_span(const AttnArgs& a, int g) {
     const int hi = !a.batch.row_begin ? e : min(max(a.batch.row_begin[e], lo), a.batch.rows);
     return {lo, hi - lo, hi - lo, a.prefix.pages + (size_t)g * a.prefix.max_pages,
             held(a.prefix.lengths[g], a.prefix.max_pages, a.kv.page_shift), 1 << 30};
+}
+
+constexpr int THREADS = 256;  // of a workgroup
+
+// The span and the row tile (of PACKED packed rows) of tile number `want` over
+// all spans, by all threads; false: there are fewer tiles.
+template <int PACKED, bool PREFIX>
+__device__ __forceinline__ bool find_tile(const AttnArgs& a, int want, int* span, int* tile) {
+    __shared__ int sums[THREADS / 64], found[2];
+    const int n = PREFIX ? a.prefix.groups : a.batch.batch, tid = threadIdx.x, lane = tid & 63;
+    if (tid == 0) found[0] = -1;
+    int before = 0;
+    for (int s0 = 0; s0 < n; s0 += THREADS) {
+        int t = 0;
+        if (s0 + tid < n) {
+            const int rows = PREFIX ? prefix_span(a, s0 + tid).count : rows_of(a.batch, s0 + tid).count;
+            t = (int)(((int64_t)rows * a.group + PACKED - 1) / PACKED);
+        }
+        int x = t;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int y = __shfl_up(x, d);
+            if (lane >= d) x += y;
+        }
+        if (lane == 63) sums[tid >> 6] = x;
+        __syncthreads();
+        int base = before, all = before;
+        for (int w = 0; w < THREADS / 64; w++) {
+            if (w < tid >> 6) base += sums[w];
+            all += sums[w];
+        }
+        const int first = base + x - t;
+        if (t > 0 && want >= first && want < first + t) found[0] = s0 + tid, found[1] = want - first;
+        __syncthreads();
+        before = all;
+        if (want < all) break;
+    }
+    *span = __builtin_amdgcn_readfirstlane(found[0]);
+    *tile = __builtin_amdgcn_readfirstlane(found[1]);
+    return *span >= 0;
 }
 
 // The page of position j (the same for the whole wave), -1 where none holds

@@ -28,7 +28,7 @@
 namespace lq8 {
 namespace {
 
-constexpr int FEW_WAVES = 4;
+constexpr int FEW_WAVES = THREADS / 64;
 
 template <int TYPES, int D> struct Tile;
 // bf16 pages
@@ -82,18 +82,15 @@ __device__ __forceinline__ void few_body(const AttnArgs& a, int block, char* sm)
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     char* own = sm + w * WBYTES;
 
-    // block -> (piece, span, row tile, kv head), kv head fastest: the blocks of
-    // one go to one XCD where their number divides by eight, and the row tiles
-    // of a piece read its pages together
+    // block -> (piece, row tile, kv head), kv head fastest: the blocks of one
+    // go to one XCD where their number divides by eight, and the row tiles of a
+    // piece read its pages at about the same time
     const Cut& cut = PREFIX ? a.pre : a.own;
     const int G = a.group, kvh = a.kv.kv_heads, tiles = PREFIX ? a.pre_few : a.own_few;
-    int x = block;
-    const int g = x % kvh;
-    x /= kvh;
-    const int row0 = x % tiles * FEW_PACKED;
-    x /= tiles;
-    const int spans = PREFIX ? a.prefix.groups : a.batch.batch;
-    const int sp = x % spans, piece = x / spans;
+    const int g = block % kvh, piece = block / kvh / tiles;
+    int sp = block / kvh % tiles, tile = 0;
+    if (!(PREFIX ? a.pre_each : a.own_each) && !find_tile<FEW_PACKED, PREFIX>(a, sp, &sp, &tile)) return;
+    const int row0 = tile * FEW_PACKED;
     const Span s = PREFIX ? prefix_span(a, sp) : own_span(a, sp);
     const int packed = min(s.count * G - row0, FEW_PACKED);
     if (packed <= 0) return;
@@ -138,20 +135,20 @@ __device__ __forceinline__ void few_body(const AttnArgs& a, int block, char* sm)
     for (int t = 0; t < DT; t++) acc[t] = v4f{0, 0, 0, 0};
     float m = -__builtin_huge_valf(), l = 0.0f;
 
-    T tile;
+    T kv;
     constexpr int BLOCKS = N / 16;
     const char *kc = (const char*)a.kv.k, *vc = (const char*)a.kv.v;
     auto load_k = [&](const size_t (&off)[BLOCKS]) {
         if constexpr (F32C) {
             const float* kp = (const float*)kc + off[0] + r * D + 4 * p;
 #pragma unroll
-            for (int t = 0; t < T::KS; t++) tile.k[t] = *(const v4f*)(kp + 16 * t);
+            for (int t = 0; t < T::KS; t++) kv.k[t] = *(const v4f*)(kp + 16 * t);
         } else {
 #pragma unroll
             for (int b = 0; b < BLOCKS; b++) {
                 const uint16_t* kp = (const uint16_t*)kc + off[b] + r * D + 8 * p;
 #pragma unroll
-                for (int t = 0; t < T::KS; t++) tile.k[b][t] = stream<TERMS == 1>(kp + 32 * t);
+                for (int t = 0; t < T::KS; t++) kv.k[b][t] = stream<TERMS == 1>(kp + 32 * t);
             }
         }
     };
@@ -161,12 +158,12 @@ __device__ __forceinline__ void few_body(const AttnArgs& a, int block, char* sm)
 #pragma unroll
             for (int v = 0; v < 4; v++)
 #pragma unroll
-                for (int h = 0; h < T::VH; h++) tile.v[v][h] = *(const v4f*)(vp + v * D + 64 * h);
+                for (int h = 0; h < T::VH; h++) kv.v[v][h] = *(const v4f*)(vp + v * D + 64 * h);
         } else {
 #pragma unroll
             for (int i = 0; i < T::VI; i++) {
                 const uint16_t* vp = (const uint16_t*)vc + off[i * T::RPI / 16] + (i * T::RPI % 16) * D + lane * 8;
-                tile.v[i] = stream<TERMS == 1>(vp);
+                kv.v[i] = stream<TERMS == 1>(vp);
             }
         }
     };
@@ -208,13 +205,13 @@ __device__ __forceinline__ void few_body(const AttnArgs& a, int block, char* sm)
 #pragma unroll
                 for (int i = 0; i < T::KS; i++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) t = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.k[i][e], qf[i][e], t, 0, 0, 0);
+                    for (int e = 0; e < 4; e++) t = __builtin_amdgcn_mfma_f32_16x16x4f32(kv.k[i][e], qf[i][e], t, 0, 0, 0);
             } else {
 #pragma unroll
                 for (int z = TERMS - 1; z >= 0; z--)
 #pragma unroll
                     for (int i = 0; i < T::KS; i++)
-                        t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, tile.k[b][i]), __builtin_bit_cast(v8b, q[z][i]), t, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, kv.k[b][i]), __builtin_bit_cast(v8b, q[z][i]), t, 0, 0, 0);
             }
             sc[b] = t;
         }
@@ -290,8 +287,8 @@ __device__ __forceinline__ void few_body(const AttnArgs& a, int block, char* sm)
                     const bool gone = hole || j + 4 * p + v >= end;
 #pragma unroll
                     for (int h = 0; h < T::VH; h++) {
-                        if (gone) tile.v[v][h] = v4f{0, 0, 0, 0};
-                        mark_odd<true>(__builtin_bit_cast(v4u, tile.v[v][h]), bits);
+                        if (gone) kv.v[v][h] = v4f{0, 0, 0, 0};
+                        mark_odd<true>(__builtin_bit_cast(v4u, kv.v[v][h]), bits);
                     }
                 }
                 odd = __any(is_odd<true>(bits));
@@ -300,7 +297,7 @@ __device__ __forceinline__ void few_body(const AttnArgs& a, int block, char* sm)
                     for (int v = 0; v < 4; v++)
 #pragma unroll
                         for (int h = 0; h < T::VH; h++)
-                            tile.v[v][h] = __builtin_bit_cast(v4f, finite_part<true>(__builtin_bit_cast(v4u, tile.v[v][h])));
+                            kv.v[v][h] = __builtin_bit_cast(v4f, finite_part<true>(__builtin_bit_cast(v4u, kv.v[v][h])));
                 }
             }
 #pragma unroll
@@ -309,29 +306,29 @@ __device__ __forceinline__ void few_body(const AttnArgs& a, int block, char* sm)
                 for (int h = 0; h < T::VH; h++)
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        acc[4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(tile.v[v][h][e], sc[0][v], acc[4 * h + e], 0, 0, 0);
+                        acc[4 * h + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv.v[v][h][e], sc[0][v], acc[4 * h + e], 0, 0, 0);
             if (jn < end) load_v(on);
         } else {
             if (masked) {
 #pragma unroll
                 for (int i = 0; i < T::VI; i++) {
                     const int row = i * T::RPI + lane / (D / 8);
-                    if (pg[i * T::RPI / 16] < 0 || j + row >= end) tile.v[i] = v4u{0, 0, 0, 0};
+                    if (pg[i * T::RPI / 16] < 0 || j + row >= end) kv.v[i] = v4u{0, 0, 0, 0};
                 }
             }
             if (masked || TERMS > 1) {
                 uint32_t bits = 0;
 #pragma unroll
-                for (int i = 0; i < T::VI; i++) mark_odd<false>(tile.v[i], bits);
+                for (int i = 0; i < T::VI; i++) mark_odd<false>(kv.v[i], bits);
                 odd = __any(is_odd<false>(bits));
                 if (odd) {
 #pragma unroll
-                    for (int i = 0; i < T::VI; i++) tile.v[i] = finite_part<false>(tile.v[i]);
+                    for (int i = 0; i < T::VI; i++) kv.v[i] = finite_part<false>(kv.v[i]);
                 }
             }
 #pragma unroll
             for (int i = 0; i < T::VI; i++)
-                *(v4u*)(own + lds_slot<2 * D>(i * T::RPI + lane / (D / 8), lane % (D / 8))) = tile.v[i];
+                *(v4u*)(own + lds_slot<2 * D>(i * T::RPI + lane / (D / 8), lane % (D / 8))) = kv.v[i];
             if (jn < end) load_v(on);
             __builtin_amdgcn_wave_barrier();
             v4u pb[TERMS];

@@ -5,14 +5,14 @@ namespace lq8 {
 namespace {
 
 template <int TYPES, int D, bool PREFIX>
-__global__ __launch_bounds__(64 * FEW_WAVES, 2) void k_few(AttnArgs a) {
+__global__ __launch_bounds__(THREADS, 2) void k_few(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) char sm[few_lds<D>()];
     few_body<TYPES, D, PREFIX>(a, blockIdx.x, sm);
 }
 
 template <int TYPES>
 void launch_types(dim3 grid, hipStream_t s, const AttnArgs& a, int dim, bool prefix) {
-    const dim3 block(64 * FEW_WAVES);
+    const dim3 block(THREADS);
     if (dim == 64 && prefix) hipLaunchKernelGGL((k_few<TYPES, 64, true>), grid, block, 0, s, a);
     else if (dim == 64) hipLaunchKernelGGL((k_few<TYPES, 64, false>), grid, block, 0, s, a);
     else if (prefix) hipLaunchKernelGGL((k_few<TYPES, 128, true>), grid, block, 0, s, a);

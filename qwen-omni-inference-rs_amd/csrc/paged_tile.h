@@ -21,46 +21,6 @@
 namespace lq8 {
 namespace {
 
-constexpr int THREADS = 256;  // of a workgroup
-
-// The span and the row tile of tile number `want` over all spans, by all
-// threads; false: there are fewer tiles.
-template <bool PREFIX>
-__device__ __forceinline__ bool find_tile(const AttnArgs& a, int want, int* span, int* tile) {
-    __shared__ int sums[THREADS / 64], found[2];
-    const int n = PREFIX ? a.prefix.groups : a.batch.batch, tid = threadIdx.x, lane = tid & 63;
-    if (tid == 0) found[0] = -1;
-    int before = 0;
-    for (int s0 = 0; s0 < n; s0 += THREADS) {
-        int t = 0;
-        if (s0 + tid < n) {
-            const int rows = PREFIX ? prefix_span(a, s0 + tid).count : rows_of(a.batch, s0 + tid).count;
-            t = (int)(((int64_t)rows * a.group + TILE_PACKED - 1) / TILE_PACKED);
-        }
-        int x = t;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int y = __shfl_up(x, d);
-            if (lane >= d) x += y;
-        }
-        if (lane == 63) sums[tid >> 6] = x;
-        __syncthreads();
-        int base = before, all = before;
-        for (int w = 0; w < THREADS / 64; w++) {
-            if (w < tid >> 6) base += sums[w];
-            all += sums[w];
-        }
-        const int first = base + x - t;
-        if (t > 0 && want >= first && want < first + t) found[0] = s0 + tid, found[1] = want - first;
-        __syncthreads();
-        before = all;
-        if (want < all) break;
-    }
-    *span = __builtin_amdgcn_readfirstlane(found[0]);
-    *tile = __builtin_amdgcn_readfirstlane(found[1]);
-    return *span >= 0;
-}
-
 // A workgroup's rows and positions.
 struct Work {
     Span s;
@@ -76,7 +36,7 @@ __device__ __forceinline__ bool find_work(const AttnArgs& a, int block, Work* k)
     k->g = block % kvh;
     k->piece = x % cut.pieces;
     int sp, tile;
-    if (!find_tile<PREFIX>(a, x / cut.pieces, &sp, &tile)) return false;
+    if (!find_tile<TILE_PACKED, PREFIX>(a, x / cut.pieces, &sp, &tile)) return false;
     k->s = PREFIX ? prefix_span(a, sp) : own_span(a, sp);
     const int rows = k->s.count * a.group;
     k->row0 = ((rows + TILE_PACKED - 1) / TILE_PACKED - 1 - tile) * TILE_PACKED;
