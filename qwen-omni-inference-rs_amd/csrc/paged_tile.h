@@ -117,8 +117,8 @@ __device__ __forceinline__ void meet_odd_tile(const AttnArgs& a, const Work& k, 
 // the same quotients, and the sums are rescaled a few times instead of often.
 constexpr float LAG = 8.0f;
 
-// LDS of a workgroup: K and V of two tiles, and a few words
-template <int TYPES, int D> constexpr int tile_lds() { return (TYPES == PT_F32_F32 ? 32 * 4 : 64 * 2) * D * 4 + 16; }
+// LDS of a workgroup: K and V of two tiles, or of one in three terms, and a few words
+template <int TYPES, int D> constexpr int tile_lds() { return (TYPES == PT_F32_F32 ? 32 * 6 : 64 * 4) * 2 * D + 16; }
 
 // Block `block` of the launch; sm: tile_lds bytes, aligned to 256.
 template <int TERMS, int D, bool PREFIX>
@@ -438,15 +438,33 @@ __device__ __forceinline__ void tile_bf16_body(const AttnArgs& a, int block, cha
     });
 }
 
+// x = the sum of three bf16 terms, exactly, for eight x: z[k] holds the terms k.
+// The first is cut (rounded it could be infinite), the second rounded, so that
+// the products of second and third terms, which are left out, have either
+// sign: 2^-24 of a product in the mean square.  What is not finite becomes NaN.
+__device__ __forceinline__ void split_terms(v4f x0, v4f x1, v4u (&z)[3]) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float a = e < 2 ? x0[2 * e] : x1[2 * e - 4], b = e < 2 ? x0[2 * e + 1] : x1[2 * e - 3];
+        const uint32_t w0 = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+        const float ra = a - low_bf16(w0), rb = b - high_bf16(w0);
+        const uint32_t w1 = pack_bf16(ra, rb);
+        z[0][e] = w0;
+        z[1][e] = w1;
+        z[2][e] = pack_bf16(ra - low_bf16(w1), rb - high_bf16(w1));
+    }
+}
+
+// f32 pages.  The float32 products run at a sixteenth of the bf16 ones' rate,
+// so every operand is split into three bf16 terms, K and V on their way into
+// LDS, and the six products of terms that count are taken.
 template <int D, bool PREFIX>
 __device__ __forceinline__ void tile_f32_body(const AttnArgs& a, int block, char* sm) {
-    constexpr int ES = 4, ROW = D * ES, N = 32;
-    constexpr int BLOCKS = N / 16, SB = N / 32;               // page blocks, score blocks of a tile
-    constexpr int CPR = ROW / 16, CI = N * CPR / THREADS;     // 16-byte chunks of a row; of a thread
-    constexpr int DT = D / 32, VW = D / 32;
-    constexpr int TB = N * ROW;
-    int& odd_lo = *(int*)(sm + 4 * TB);  // positions of tiles with values that are not finite
-    int& odd_hi = *(int*)(sm + 4 * TB + 4);
+    constexpr int ROW = 2 * D, N = 32, PB = N * ROW;  // a plane: one term of K or V; K's three, then V's
+    constexpr int TPR = D / 8, RPN = THREADS / TPR, CI = N / RPN;  // eight values a thread; rows of a step; steps
+    constexpr int DT = D / 32, KS = D / 16;
+    int& odd_lo = *(int*)(sm + 6 * PB);  // positions of tiles with values that are not finite
+    int& odd_hi = *(int*)(sm + 6 * PB + 4);
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, p = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
@@ -457,15 +475,11 @@ __device__ __forceinline__ void tile_f32_body(const AttnArgs& a, int block, char
     if (tid == 0) odd_lo = INT32_MAX, odd_hi = 0;
     const LaneRow me(a, wk, w, r);
     const size_t qat = me.row * a.qs + (size_t)me.head * D;
-    float qf[D / 2];
+    v4u q[KS][3];
     {
-        const float* qp = (const float*)a.q + qat + 4 * p;
+        const float* qp = (const float*)a.q + qat + 8 * p;
 #pragma unroll
-        for (int t = 0; t < D / 8; t++) {
-            const v4f v = *(const v4f*)(qp + 8 * t);
-#pragma unroll
-            for (int e = 0; e < 4; e++) qf[4 * t + e] = v[e];
-        }
+        for (int t = 0; t < KS; t++) split_terms(*(const v4f*)(qp + 16 * t), *(const v4f*)(qp + 16 * t + 4), q[t]);
     }
 
     v16f acc[DT];
@@ -473,60 +487,55 @@ __device__ __forceinline__ void tile_f32_body(const AttnArgs& a, int block, char
     for (int t = 0; t < DT; t++)
 #pragma unroll
         for (int e = 0; e < 16; e++) acc[t][e] = 0.0f;
-    float m = -__builtin_huge_valf(), l = 0.0f;
+    float m = -__builtin_huge_valf(), l = 0.0f, mu = -FLT_MAX;
+    bool far = false;
 
-    // staging: chunk tid + 256 n of the tile; a wave's rows lie in one block
-    v4u kr[CI], vr[CI];
-    int pg[BLOCKS], pn[BLOCKS];  // of this tile and the next
-    const char *kc = (const char*)a.kv.k, *vc = (const char*)a.kv.v;
-    auto pages_of = [&](int j, int (&pg)[BLOCKS]) {
-#pragma unroll
-        for (int b = 0; b < BLOCKS; b++) pg[b] = page_at(a, s, j + 16 * b, end);
-    };
-    constexpr int RPN = THREADS / CPR;  // rows of a step
-    auto page_of = [&](const int (&pg)[BLOCKS], int n) {  // of the wave's rows of step n
-        if constexpr (RPN <= 16) return pg[n * RPN / 16];
-        else return w >= 2 ? pg[2 * n + 1] : pg[2 * n];
-    };
-    const int lane_at = (tid / CPR & 15) * ROW + tid % CPR * 16;
-    auto load = [&](const int (&pg)[BLOCKS], int j) {
+    // staging: values 8 (tid % TPR) .. of row tid / TPR + RPN n of the tile
+    v4f kr[CI][2], vr[CI][2];
+    int pg[2], pn[2];  // pages of this tile's blocks and the next's
+    auto pages_of = [&](int j, int (&pg)[2]) { pg[0] = page_at(a, s, j, end), pg[1] = page_at(a, s, j + 16, end); };
+    const float *kc = (const float*)a.kv.k, *vc = (const float*)a.kv.v;
+    auto page_of = [&](const int (&pg)[2], int n) { return RPN == 16 ? pg[n] : w >= 2 ? pg[1] : pg[0]; };
+    const int lane_at = (tid / TPR & 15) * D + tid % TPR * 8;
+    auto load = [&](const int (&pg)[2], int j) {
 #pragma unroll
         for (int n = 0; n < CI; n++) {
-            const int b = RPN <= 16 ? n * RPN / 16 : 2 * n + w / 2;
-            const size_t at = slot_off(a, page_of(pg, n), g, j + 16 * b, D) * ES;
-            const int o = lane_at + (RPN < 16 ? n * RPN % 16 * ROW : 0);
-            kr[n] = *(const v4u*)(kc + at + o);
-            vr[n] = *(const v4u*)(vc + at + o);
+            const size_t at = slot_off(a, page_of(pg, n), g, j + 16 * (RPN == 16 ? n : w / 2), D) + lane_at;
+            kr[n][0] = *(const v4f*)(kc + at), kr[n][1] = *(const v4f*)(kc + at + 4);
+            vr[n][0] = *(const v4f*)(vc + at), vr[n][1] = *(const v4f*)(vc + at + 4);
         }
     };
-    // registers -> buffer `buf`, the tile at position j.  Values of rows
-    // that no row sees become zeros, and so does what is not finite where
-    // some row must not meet it (fixed up after the products).
-    const int least = s.sees(wk.row0 / a.group);
-    auto store = [&](int buf, int j, const int (&pg)[BLOCKS]) {
-        bool hole = false;
+    // registers -> LDS, the tile at position j.  Values of rows that no row
+    // sees become zeros, and so does what is not finite (meet_odd).
+    auto store = [&](int j, const int (&pg)[2]) {
+        uint32_t bits = 0;
 #pragma unroll
-        for (int b = 0; b < BLOCKS; b++) hole |= pg[b] < 0;
-        const bool check = hole || j + N > least;
-        if (check) {
-            uint32_t bits = 0;
+        for (int n = 0; n < CI; n++) {
+            const bool gone = page_of(pg, n) < 0 || j + n * RPN + tid / TPR >= end;
 #pragma unroll
-            for (int n = 0; n < CI; n++) {
-                if (page_of(pg, n) < 0 || j + n * RPN + tid / CPR >= end) vr[n] = v4u{0, 0, 0, 0};
-                mark_odd<true>(vr[n], bits);
+            for (int h = 0; h < 2; h++) {
+                if (gone) vr[n][h] = v4f{0, 0, 0, 0};
+                mark_odd<true>(__builtin_bit_cast(v4u, vr[n][h]), bits);
             }
-            if (is_odd<true>(bits)) {
-                atomicMin(&odd_lo, j);
-                atomicMax(&odd_hi, j + N);
+        }
+        if (is_odd<true>(bits)) {
+            atomicMin(&odd_lo, j);
+            atomicMax(&odd_hi, j + N);
 #pragma unroll
-                for (int n = 0; n < CI; n++) vr[n] = finite_part<true>(vr[n]);
-            }
+            for (int n = 0; n < CI; n++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) vr[n][h] = __builtin_bit_cast(v4f, finite_part<true>(__builtin_bit_cast(v4u, vr[n][h])));
         }
 #pragma unroll
         for (int n = 0; n < CI; n++) {
-            const int at = lds_slot<ROW>(n * RPN + tid / CPR, tid % CPR);
-            *(v4u*)(sm + 2 * TB * buf + at) = kr[n];
-            *(v4u*)(sm + 2 * TB * buf + TB + at) = vr[n];
+            char* at = sm + lds_slot<ROW>(n * RPN + tid / TPR, tid % TPR);
+            v4u z[3];
+            split_terms(kr[n][0], kr[n][1], z);
+#pragma unroll
+            for (int y = 0; y < 3; y++) *(v4u*)(at + y * PB) = z[y];
+            split_terms(vr[n][0], vr[n][1], z);
+#pragma unroll
+            for (int y = 0; y < 3; y++) *(v4u*)(at + (3 + y) * PB) = z[y];
         }
     };
 
@@ -536,123 +545,143 @@ __device__ __forceinline__ void tile_f32_body(const AttnArgs& a, int block, char
         pages_of(j + N, pn);
         load(pg, j);
         __syncthreads();  // odd_lo, odd_hi are set up
-        store(0, j, pg);
+        store(j, pg);
+        __syncthreads();
     }
 #pragma unroll
-    for (int t = 0; t < D / 2; t++) arrived(qf[t]);
-    for (int k = 0; j < end; k++, j += N) {
-        const int buf = k & 1, jn = j + N;
-        __syncthreads();
+    for (int t = 0; t < KS; t++)
+#pragma unroll
+        for (int z = 0; z < 3; z++) arrived(q[t][z]);
+    for (; j < end; j += N) {
+        const int jn = j + N;
         if (jn < end) load(pn, jn);
-        int pnn[BLOCKS];  // a tile ahead of its loads
+        int pnn[2];  // a tile ahead of its loads
         pages_of(jn + N, pnn);
         if (j < me.most) {
-            const char *K = sm + 2 * TB * buf, *V = K + TB;
-            v16f sc[SB];
+            // scores, K's operands a step ahead; lds_slot(r, 2 c + p) = lds_slot(r, p) ^ 32 c
+            v16f sc;
+            {
+                int at = lds_slot<ROW>(r, p);
+                asm volatile("" : "+v"(at));
+                v8b ko[2][3];
+                auto load_k = [&](int c) {
 #pragma unroll
-            for (int b = 0; b < SB; b++) {
-                v16f t;
+                    for (int y = 0; y < 3; y++) ko[c % 2][y] = *(const v8b*)(sm + y * PB + (at ^ (c << 5)));
+                };
+                load_k(0);
 #pragma unroll
-                for (int e = 0; e < 16; e++) t[e] = 0.0f;
+                for (int e = 0; e < 16; e++) sc[e] = 0.0f;
 #pragma unroll
-                for (int c = 0; c < D / 8; c++) {
-                    const v4f kv = *(const v4f*)(K + lds_slot<ROW>(32 * b + r, 2 * c + p));
+                for (int c = 0; c < KS; c++) {
+                    if (c + 1 < KS) load_k(c + 1);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) t = __builtin_amdgcn_mfma_f32_32x32x2f32(kv[e], qf[4 * c + e], t, 0, 0, 0);
+                    for (int o = 2; o >= 0; o--)
+#pragma unroll
+                        for (int y = 0; y <= o; y++)
+                            sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ko[c % 2][y], __builtin_bit_cast(v8b, q[c][o - y]), sc, 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                sc[b] = t;
             }
-            bool hole = false;
-#pragma unroll
-            for (int b = 0; b < BLOCKS; b++) hole |= pg[b] < 0;
-            const bool masked = hole || j + N > me.least || !me.whole;
-            // element e of block b: position 32 b + 8 (e / 4) + 4 p + e % 4
-            auto seen = [&](int b, int e) { return pg[2 * b + e / 8] >= 0 && j + 32 * b + 8 * (e / 4) + 4 * p + e % 4 < me.sees; };
+            const bool masked = pg[0] < 0 || pg[1] < 0 || j + N > me.least || !me.whole;
+            // element e: position 8 (e / 4) + 4 p + e % 4
+            float mx = -FLT_MAX;
             if (masked) {
+                mx = -__builtin_huge_valf();
 #pragma unroll
-                for (int b = 0; b < SB; b++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) sc[b][e] = seen(b, e) ? sc[b][e] : -__builtin_huge_valf();
+                for (int e = 0; e < 16; e++) {
+                    const bool seen = pg[e / 8] >= 0 && j + 8 * (e / 4) + 4 * p + e % 4 < me.sees;
+                    sc[e] = seen ? sc[e] : -__builtin_huge_valf();
+                    mx = seen ? -FLT_MAX : mx;
+                }
             }
-            float mx = masked ? -__builtin_huge_valf() : -FLT_MAX;
-            if (masked) {
+            {
+                // terms of what is not finite, or infinite products of terms: such scores again, product by product
+                float sum = 0.0f;
 #pragma unroll
-                for (int b = 0; b < SB; b++)
+                for (int e = 0; e < 16; e++) sum += sc[e];
+                if (__any(sum != sum)) {
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const float y = sc[b][e] * a.c;
-                        mx = fmaxf(mx, seen(b, e) ? fmaxf(y, -FLT_MAX) : y);
-                    }
-            } else {
+                    for (int e = 0; e < 16; e++)
+                        if (sc[e] != sc[e]) {
+                            const float* qp = (const float*)a.q + qat;
+                            const float* kp = kc + slot_off(a, pg[e / 8], g, j + 16 * (e / 8), D) + (8 * (e / 4 % 2) + 4 * p + e % 4) * D;
+                            float t = 0.0f;
+                            for (int d = 0; d < D; d++) t = fmaf(qp[d], kp[d], t);
+                            sc[e] = t;
+                        }
+                }
+            }
+            {
                 // (c > 0: the largest score scaled is the largest scaled score)
-                float y = sc[0][0];
+                float y = sc[0];
 #pragma unroll
-                for (int b = 0; b < SB; b++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) y = fmaxf(y, sc[b][e]);
+                for (int e = 1; e < 16; e++) y = fmaxf(y, sc[e]);
                 mx = fmaxf(mx, y * a.c);
             }
             mx = fmaxf(mx, lane_xor<32>(mx));
-            const float mn = fmaxf(m, mx), mu = fmaxf(mn, -FLT_MAX);
-            if (__any(mn != m)) {
-                const float al = __builtin_amdgcn_exp2f(m - mu);
-                l *= al;
-#pragma unroll
-                for (int t = 0; t < DT; t++) acc[t] *= al;
+            float al = 1.0f;
+            if (__any(mx > m + LAG)) {
+                const float mn = fmaxf(m, mx);
+                mu = fmaxf(mn, -FLT_MAX);
+                al = __builtin_amdgcn_exp2f(m - mu);
+                m = mn;
+                far = __any(far_score(mu));
             }
-            m = mn;
-            const bool far = __any(far_score(mu));
+            l *= al;
+#pragma unroll
+            for (int t = 0; t < DT; t++) acc[t] *= al;
             if (far) {
 #pragma unroll
-                for (int b = 0; b < SB; b++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) sc[b][e] = sc[b][e] * a.c - mu;
+                for (int e = 0; e < 16; e++) sc[e] = __builtin_amdgcn_exp2f(sc[e] * a.c - mu);
             } else {
 #pragma unroll
-                for (int b = 0; b < SB; b++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) sc[b][e] = fmaf(sc[b][e], a.c, -mu);
+                for (int e = 0; e < 16; e++) sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.c, -mu));
             }
 #pragma unroll
-            for (int b = 0; b < SB; b++)
+            for (int e = 0; e < 16; e++) l += sc[e];
+            // lds_slot(16 ks + 8 h + row, ch + 4 t) = (lds_slot(row, ch) ^ 64 t ^ 32 h) + (16 ks + 8 h) ROW
+            int vat = 3 * PB + lds_slot<ROW>(4 * p + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 8 * (lane & 1);
+            asm volatile("" : "+v"(vat));
+            v8b vo[2][3];
+            auto load_v = [&](int i) {
+                const int ks = i / DT, t = i % DT;
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    sc[b][e] = __builtin_amdgcn_exp2f(sc[b][e]);
-                    l += sc[b][e];
+                for (int y = 0; y < 3; y++) {
+                    const char* at = sm + y * PB + 16 * ks * ROW;
+                    vo[i % 2][y] = join_halves(read_transposed(at + (vat ^ (t << 6))), read_transposed(at + 8 * ROW + (vat ^ (t << 6) ^ 32)));
                 }
-            {
+            };
+            load_v(0);
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int vrow = 8 * (e / 4) + 4 * p + e % 4;
-                    v4f v;
-                    if constexpr (VW == 4) {
-                        v = *(const v4f*)(V + lds_slot<ROW>(vrow, r));
-                    } else {
-                        const float2 two = *(const float2*)(V + lds_slot<ROW>(vrow, r >> 1) + 8 * (r & 1));
-                        v = v4f{two.x, two.y, 0.0f, 0.0f};
-                    }
+            for (int ks = 0; ks < 2; ks++) {
+                v4u pb[3];
+                split_terms(v4f{sc[8 * ks], sc[8 * ks + 1], sc[8 * ks + 2], sc[8 * ks + 3]}, v4f{sc[8 * ks + 4], sc[8 * ks + 5], sc[8 * ks + 6], sc[8 * ks + 7]}, pb);
 #pragma unroll
-                    for (int t = 0; t < DT; t++) acc[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[t], sc[0][e], acc[t], 0, 0, 0);
+                for (int t = 0; t < DT; t++) {
+                    const int i = ks * DT + t;
+                    if (i + 1 < 2 * DT) load_v(i + 1);
+#pragma unroll
+                    for (int o = 2; o >= 0; o--)
+#pragma unroll
+                        for (int y = 0; y <= o; y++)
+                            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vo[i % 2][y], __builtin_bit_cast(v8b, pb[o - y]), acc[t], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
-        if (jn < end) store(buf ^ 1, jn, pn);
-#pragma unroll
-        for (int b = 0; b < BLOCKS; b++) pg[b] = pn[b], pn[b] = pnn[b];
+        __syncthreads();
+        if (jn < end) store(jn, pn);
+        __syncthreads();
+        pg[0] = pn[0], pg[1] = pn[1], pn[0] = pnn[0], pn[1] = pnn[1];
     }
 
     __syncthreads();
-    if (odd_hi) meet_odd_tile<float, float, D>(a, wk, me, qat, odd_lo, odd_hi, m, [&](int t, int e) { return VW * (8 * (e / 4) + 4 * p + e % 4) + t; }, acc);
+    if (odd_hi) meet_odd_tile<float, float, D>(a, wk, me, qat, odd_lo, odd_hi, m, [&](int t, int e) { return 32 * t + 8 * (e / 4) + 4 * p + e % 4; }, acc);
     finish<true, D, PREFIX>(a, wk, me, p, m, l, [&](auto put) {
-        if constexpr (VW == 4) {
 #pragma unroll
-            for (int e = 0; e < 16; e++)
-                put(4 * (8 * (e / 4) + 4 * p + e % 4), v4f{acc[0][e], acc[1 % DT][e], acc[2 % DT][e], acc[3 % DT][e]});
-        } else {
+        for (int t = 0; t < DT; t++)
 #pragma unroll
-            for (int e = 0; e < 16; e += 2)
-                put(2 * (8 * (e / 4) + 4 * p + e % 4), v4f{acc[0][e], acc[1][e], acc[0][e + 1], acc[1][e + 1]});
-        }
+            for (int e = 0; e < 16; e += 4) put(32 * t + 2 * e + 4 * p, v4f{acc[t][e], acc[t][e + 1], acc[t][e + 2], acc[t][e + 3]});
     });
 }
 
