@@ -172,10 +172,11 @@ Cut cut_of(size_t most, size_t groups, int cus, bool few, bool f32_pages, float 
 //     packed                32            48            64            96
 //     bf16                  42 /  23      52 /  27      61 /  26      80 /  29
 //     f32 over bf16         42 /  37      47 /  45      57 /  45      69 /  48
-//     f32                   58 /  82      80 / 120      98 / 115     133 / 118
-// and 32 x 2000: f32 over bf16 55 / 64, 67 / 86, 82 / 86, 112 / 90.  Where the
-// blocks of 16 rows by a piece are at most two a compute unit, latency decides:
-// 1 x 2000 of bf16 11 / 15, 13 / 17, 14 / 16 and (three a unit) 18 / 18.
+//     f32                   60 /  68      67 /  72      74 /  71     133 /  74
+// and 32 x 2000: f32 over bf16 55 / 64, 67 / 86, 82 / 86, 112 / 90; f32 87 /
+// 138, 116 / 160, 137 / 160, 243 / 168.  Where the blocks of 16 rows by a piece
+// are at most two a compute unit, latency decides: 1 x 2000 of bf16 11 / 15,
+// 13 / 17, 14 / 16 and (three a unit) 18 / 18.
 bool takes_few(PagedTypes types, size_t packed, size_t blocks, int cus) {
     return packed <= (types == PT_BF16_BF16 ? 16 : types == PT_F32_BF16 ? 48 : 64) || blocks <= 2 * (size_t)cus;
 }

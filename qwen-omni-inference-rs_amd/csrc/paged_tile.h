@@ -2,16 +2,15 @@
 // head: prompt chunks, and the rows of a group that share a prefix (gfx950).
 //
 // A workgroup has 128 packed rows, 32 to a wave, and goes over its piece in
-// tiles of 64 positions (bf16 pages) or 32 (f32), K and V in LDS, two buffers:
-// the next tile's loads are out while this one is computed, one barrier a tile.
+// tiles of 64 positions (bf16 pages: K and V in LDS, two buffers, the next
+// tile's loads out while this one is computed) or 32 (f32 pages, one buffer).
 // The rows are the columns of the products (32 x 32 tiles): S^T = K Q^T leaves
 // lane (row = lane % 32, p = lane / 32) with the scores of positions 8 i + 4 p
 // .. + 3 of its row, which is the B operand of O^T = V^T P^T when the 16
 // positions of a product are taken in the order (4 p + e, 8 + 4 p + e): the
 // probabilities stay where they are, the maximum needs one exchange with lane
 // +- 32, and the rescaling of O none.  V is read transposed (ds_read_tr).
-// f32 pages: 32 x 32 x 2 products on float32 operands.  f32 rows over bf16
-// pages: three bf16 terms of q and p each, as in paged_few.hip.
+// f32 rows: three bf16 terms of q and p each; f32 pages: of K and V too.
 #pragma once
 
 #include <type_traits>
@@ -457,7 +456,10 @@ __device__ __forceinline__ void split_terms(v4f x0, v4f x1, v4u (&z)[3]) {
 
 // f32 pages.  The float32 products run at a sixteenth of the bf16 ones' rate,
 // so every operand is split into three bf16 terms, K and V on their way into
-// LDS, and the six products of terms that count are taken.
+// LDS, and the six products of terms that count are taken: 138 us for 951 rows
+// over 2999 positions, 16 heads over 8 of 128 (19.7 GFLOP), against 222 with
+// float32 products (152.8 TFLOP/s at most).  One tile in LDS, so that two
+// workgroups share a compute unit and one computes while the other splits.
 template <int D, bool PREFIX>
 __device__ __forceinline__ void tile_f32_body(const AttnArgs& a, int block, char* sm) {
     constexpr int ROW = 2 * D, N = 32, PB = N * ROW;  // a plane: one term of K or V; K's three, then V's
@@ -558,7 +560,8 @@ __device__ __forceinline__ void tile_f32_body(const AttnArgs& a, int block, char
         int pnn[2];  // a tile ahead of its loads
         pages_of(jn + N, pnn);
         if (j < me.most) {
-            // scores, K's operands a step ahead; lds_slot(r, 2 c + p) = lds_slot(r, p) ^ 32 c
+            // scores, K's operands a step ahead, products in two chains (138 us
+            // against 141); lds_slot(r, 2 c + p) = lds_slot(r, p) ^ 32 c
             v16f sc;
             {
                 int at = lds_slot<ROW>(r, p);
@@ -571,16 +574,20 @@ __device__ __forceinline__ void tile_f32_body(const AttnArgs& a, int block, char
                 load_k(0);
 #pragma unroll
                 for (int e = 0; e < 16; e++) sc[e] = 0.0f;
+                v16f lo = sc;
 #pragma unroll
                 for (int c = 0; c < KS; c++) {
                     if (c + 1 < KS) load_k(c + 1);
-#pragma unroll
-                    for (int o = 2; o >= 0; o--)
-#pragma unroll
-                        for (int y = 0; y <= o; y++)
-                            sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ko[c % 2][y], __builtin_bit_cast(v8b, q[c][o - y]), sc, 0, 0, 0);
+                    auto mul = [&](v16f& to, int y, int z) { to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ko[c % 2][y], __builtin_bit_cast(v8b, q[c][z]), to, 0, 0, 0); };
+                    mul(lo, 0, 2);
+                    mul(sc, 0, 1);
+                    mul(lo, 1, 1);
+                    mul(sc, 1, 0);
+                    mul(lo, 2, 0);
+                    mul(sc, 0, 0);
                     __builtin_amdgcn_sched_barrier(0);
                 }
+                sc += lo;
             }
             const bool masked = pg[0] < 0 || pg[1] < 0 || j + N > me.least || !me.whole;
             // element e: position 8 (e / 4) + 4 p + e % 4
