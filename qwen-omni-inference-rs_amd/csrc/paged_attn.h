@@ -174,6 +174,11 @@ __device__ __forceinline__ v8b join_halves(v4s a, v4s b) {
 // waited for there, and with it, loads returning in order, the loop's own.
 template <typename T> __device__ __forceinline__ void arrived(T& x) { asm volatile("" : "+v"(x)); }
 
+// A row's reference m lies this far above its largest scaled score, so that
+// sums of up to 2^16 values weighted 2^(s - m) cannot pass float32's range where
+// their mean does not (2^8 of it goes to references that lag behind).
+constexpr float ABOVE = 24.0f;
+
 // Where the largest scaled score is this large, its rounding (2^-24 of it,
 // which s c - m in one fma leaves in the exponent: the same factor for every
 // position, but one that can leave the range) is taken off by rounding s c too.

@@ -259,7 +259,7 @@ __device__ __forceinline__ void few_body(const AttnArgs& a, int block, char* sm)
             }
         mx = fmaxf(mx, lane_xor<16>(mx));
         mx = fmaxf(mx, lane_xor<32>(mx));
-        const float mn = fmaxf(m, mx), mu = fmaxf(mn, -FLT_MAX);
+        const float mn = fmaxf(m, mx + ABOVE), mu = fmaxf(mn, -FLT_MAX);
         if (__any(mn != m)) {
             const float al = __builtin_amdgcn_exp2f(m - mu);
             l *= al;

@@ -358,8 +358,8 @@ __device__ __forceinline__ void tile_bf16_body(const AttnArgs& a, int block, cha
             }
             mx = fmaxf(mx, lane_xor<32>(mx));
             float al = 1.0f;
-            if (__any(mx > m + LAG)) {
-                const float mn = fmaxf(m, mx);
+            if (__any(mx > m - (ABOVE - LAG))) {
+                const float mn = fmaxf(m, mx + ABOVE);
                 mu = fmaxf(mn, -FLT_MAX);
                 al = __builtin_amdgcn_exp2f(m - mu);
                 m = mn;
@@ -627,8 +627,8 @@ __device__ __forceinline__ void tile_f32_body(const AttnArgs& a, int block, char
             }
             mx = fmaxf(mx, lane_xor<32>(mx));
             float al = 1.0f;
-            if (__any(mx > m + LAG)) {
-                const float mn = fmaxf(m, mx);
+            if (__any(mx > m - (ABOVE - LAG))) {
+                const float mn = fmaxf(m, mx + ABOVE);
                 mu = fmaxf(mn, -FLT_MAX);
                 al = __builtin_amdgcn_exp2f(m - mu);
                 m = mn;
