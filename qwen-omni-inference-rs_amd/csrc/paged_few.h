@@ -267,7 +267,7 @@ __device__ __forceinline__ void few_body(const AttnArgs& a, int block, char* sm)
             for (int t = 0; t < DT; t++) acc[t] *= al;
         }
         m = mn;
-        const bool far = __any(far_score(mu));
+        const bool far = far_score(mu);
 #pragma unroll
         for (int b = 0; b < BLOCKS; b++)
 #pragma unroll

@@ -112,7 +112,7 @@ __device__ __forceinline__ void meet_odd_tile(const AttnArgs& a, const Work& k, 
 }
 
 // The running reference of a row's exponents.  It follows the largest score
-// only when that passes it by 2^8 (somewhere in the wave): any reference gives
+// only when that passes it by 2^8: any reference gives
 // the same quotients, and the sums are rescaled a few times instead of often.
 constexpr float LAG = 8.0f;
 
@@ -359,7 +359,8 @@ __device__ __forceinline__ void tile_bf16_body(const AttnArgs& a, int block, cha
             mx = fmaxf(mx, lane_xor<32>(mx));
             float al = 1.0f;
             if (__any(mx > m - (ABOVE - LAG))) {
-                const float mn = fmaxf(m, mx + ABOVE);
+                // (of the rows that need it: a row's result is not to depend on others)
+                const float mn = mx > m - (ABOVE - LAG) ? fmaxf(m, mx + ABOVE) : m;
                 mu = fmaxf(mn, -FLT_MAX);
                 al = __builtin_amdgcn_exp2f(m - mu);
                 m = mn;
@@ -371,16 +372,15 @@ __device__ __forceinline__ void tile_bf16_body(const AttnArgs& a, int block, cha
 #pragma unroll
             for (int t = 0; t < DT; t++) acc[t] *= al;
             if (far) {
+                const float f = far_score(mu) ? a.c : 1.0f;
 #pragma unroll
-                for (int b = 0; b < SB; b++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) sc[b][e] = __builtin_amdgcn_exp2f(sc[b][e] * a.c - mu);
-            } else {
-#pragma unroll
-                for (int b = 0; b < SB; b++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) sc[b][e] = __builtin_amdgcn_exp2f(fmaf(sc[b][e], a.c, -mu));
+                for (int b = 0; b < SB; b++) sc[b] *= f;
             }
+            const float c = far && far_score(mu) ? 1.0f : a.c;
+#pragma unroll
+            for (int b = 0; b < SB; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) sc[b][e] = __builtin_amdgcn_exp2f(fmaf(sc[b][e], c, -mu));
             // lds_slot(16 ks + 8 h + row, ch + 4 t) = (lds_slot(row, ch) ^ 64 t ^ 32 h) + (16 ks + 8 h) ROW
             int vat = (2 + buf) * TB + lds_slot<ROW>(4 * p + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 8 * (lane & 1);
             asm volatile("" : "+v"(vat));
@@ -628,7 +628,8 @@ __device__ __forceinline__ void tile_f32_body(const AttnArgs& a, int block, char
             mx = fmaxf(mx, lane_xor<32>(mx));
             float al = 1.0f;
             if (__any(mx > m - (ABOVE - LAG))) {
-                const float mn = fmaxf(m, mx + ABOVE);
+                // (of the rows that need it: a row's result is not to depend on others)
+                const float mn = mx > m - (ABOVE - LAG) ? fmaxf(m, mx + ABOVE) : m;
                 mu = fmaxf(mn, -FLT_MAX);
                 al = __builtin_amdgcn_exp2f(m - mu);
                 m = mn;
@@ -637,13 +638,10 @@ __device__ __forceinline__ void tile_f32_body(const AttnArgs& a, int block, char
             l *= al;
 #pragma unroll
             for (int t = 0; t < DT; t++) acc[t] *= al;
-            if (far) {
+            if (far) sc *= far_score(mu) ? a.c : 1.0f;
+            const float c = far && far_score(mu) ? 1.0f : a.c;
 #pragma unroll
-                for (int e = 0; e < 16; e++) sc[e] = __builtin_amdgcn_exp2f(sc[e] * a.c - mu);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; e++) sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.c, -mu));
-            }
+            for (int e = 0; e < 16; e++) sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], c, -mu));
 #pragma unroll
             for (int e = 0; e < 16; e++) l += sc[e];
             // lds_slot(16 ks + 8 h + row, ch + 4 t) = (lds_slot(row, ch) ^ 64 t ^ 32 h) + (16 ks + 8 h) ROW

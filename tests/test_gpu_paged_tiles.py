@@ -155,3 +155,20 @@ def test_the_same_pages_in_several_sequences(ctx):
     b.k[2], b.v[2] = (np.concatenate([x[:16], y[32:48], x[:16], x[80:96], y[:16], x[48:58]]) for x, y in ((k0, k1), (v0, v1)))
     out, tol = b.want()
     compare(got[:b.rows], out, tol)
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_rows_result_does_not_depend_on_its_group(ctx, types, dim):
+    """Bit for bit, with the other rows of its tiles far larger, and not finite."""
+    def batch():
+        return Batch(ctx, types, [(1, 1 + 7 * i % 90) for i in range(90)], 8, 2, dim, 16, groups=([0, 90], [2011]), seed=13)
+
+    a, b = batch(), batch()
+    assert plan(ctx, a) == (16, 128)
+    b.q[1:40] = rounded(b.q[1:40] * 30, types[0])
+    b.q[40:60] = rounded(b.q[40:60] * 1e7, types[0])
+    b.q[70:75] = np.inf
+    x, y = a.run(), b.run()
+    same = np.r_[0, 60:70, 75:90]
+    assert np.isfinite(x[same]).all() and np.array_equal(x[same], y[same])
