@@ -139,8 +139,9 @@ struct Plan {
 // positions (PRE_FILL) leave these half the machine, and fewer pieces are less
 // to join: 64 rows behind 8192 positions 64, 45, 45, 49 and 59 us at 0.25, 0.5,
 // 0.75, 1 and 2.  Tiles alone: a chunk of f32 243, 222 and 233 us at 1, 2 and 4.
-// Few rows: 206, 204 and 203 us at 4, 8 and 16 (64 sequences of bf16).
-constexpr float FEW_FILL = 8, TILE_FILL = 2, PRE_FILL = 0.5f;
+// Few rows alone: 64 sequences of bf16 198, 198 and 193 us at 4, 8 and 16; with
+// a prefix the same 64 rows 45, 45, 45 and 48 us at 2, 4, 8 and 16.
+constexpr float FEW_FILL = 16, FEW_PRE_FILL = 4, TILE_FILL = 2, PRE_FILL = 0.5f;
 
 size_t few_unit(bool f32_pages) { return f32_pages ? 64 : 128; }  // a tile for each of the four waves
 
@@ -154,7 +155,7 @@ Cut cut_of(size_t most, size_t groups, int cus, bool few, bool f32_pages, float 
         c.unit = few_unit(f32_pages);
         c.shortest = c.unit;
         const size_t longest = (most + 2047) / 2048, cap = 32768 / groups;
-        pieces = std::max((size_t)(FEW_FILL * cus) / groups, std::min(longest, cap));
+        pieces = std::max((size_t)(fill * cus) / groups, std::min(longest, cap));
     } else {
         c.unit = f32_pages ? 32 : 64;
         c.shortest = 256;
@@ -186,7 +187,7 @@ Plan plan_of(AttnArgs* a, PagedTypes types, int dim, int cus) {
     const size_t G = a->group, kvh = a->kv.kv_heads, rows = a->batch.rows, batch = a->batch.batch;
     const bool f32 = types == PT_F32_F32;
     // row tiles of `spans` spans that have `all` rows together, at most `most` each and `usual` by the rule's reckoning
-    auto part = [&](size_t spans, size_t all, size_t most, size_t usual, uint32_t pages, Cut* cut, int* few, bool* one, float fill) {
+    auto part = [&](size_t spans, size_t all, size_t most, size_t usual, uint32_t pages, Cut* cut, int* few, bool* one, float few_fill, float tile_fill) {
         const size_t positions = (size_t)pages << a->kv.page_shift, units = (positions + few_unit(f32) - 1) / few_unit(f32);
         auto tiles_of = [&](size_t rows) {
             return std::min(spans * ((most * G + rows - 1) / rows), (all * G + (rows - 1) * std::min(spans, all)) / rows);
@@ -196,14 +197,14 @@ Plan plan_of(AttnArgs* a, PagedTypes types, int dim, int cus) {
         const bool is_few = takes_few(types, usual * G, tiles * kvh * units, cus);
         *few = is_few ? (int)tiles : 0;
         if (!is_few) tiles = tiles_of(TILE_PACKED);
-        *cut = cut_of(positions, tiles * kvh, cus, is_few, f32, fill);
+        *cut = cut_of(positions, tiles * kvh, cus, is_few, f32, is_few ? few_fill : tile_fill);
         return tiles * kvh * cut->pieces;
     };
-    p.own_blocks = part(batch, rows, a->batch.max_rows, a->batch.max_rows, a->batch.max_pages, &a->own, &a->own_few, &a->own_each, TILE_FILL);
+    p.own_blocks = part(batch, rows, a->batch.max_rows, a->batch.max_rows, a->batch.max_pages, &a->own, &a->own_few, &a->own_each, a->prefix.groups ? FEW_PRE_FILL : FEW_FILL, TILE_FILL);
     p.slots = a->own.pieces;
     if (a->prefix.groups) {
         const size_t groups = a->prefix.groups;  // (each may have all rows)
-        p.pre_blocks = part(groups, rows, rows, (rows + groups - 1) / groups, a->prefix.max_pages, &a->pre, &a->pre_few, &a->pre_each, a->own_few ? PRE_FILL : TILE_FILL);
+        p.pre_blocks = part(groups, rows, rows, (rows + groups - 1) / groups, a->prefix.max_pages, &a->pre, &a->pre_few, &a->pre_each, FEW_PRE_FILL, a->own_few ? PRE_FILL : TILE_FILL);
         p.slots += a->pre.pieces;
     }
     if (p.slots > 1) p.scratch = p.slots * rows * a->heads * (dim * sizeof(float) + sizeof(float2));

@@ -372,15 +372,17 @@ __device__ __forceinline__ void tile_bf16_body(const AttnArgs& a, int block, cha
 #pragma unroll
             for (int t = 0; t < DT; t++) acc[t] *= al;
             if (far) {
-                const float f = far_score(mu) ? a.c : 1.0f;
+                const float f = far_score(mu) ? a.c : 1.0f, c = far_score(mu) ? 1.0f : a.c;
 #pragma unroll
-                for (int b = 0; b < SB; b++) sc[b] *= f;
+                for (int b = 0; b < SB; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) sc[b][e] = __builtin_amdgcn_exp2f(fmaf(sc[b][e] * f, c, -mu));
+            } else {
+#pragma unroll
+                for (int b = 0; b < SB; b++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) sc[b][e] = __builtin_amdgcn_exp2f(fmaf(sc[b][e], a.c, -mu));
             }
-            const float c = far && far_score(mu) ? 1.0f : a.c;
-#pragma unroll
-            for (int b = 0; b < SB; b++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) sc[b][e] = __builtin_amdgcn_exp2f(fmaf(sc[b][e], c, -mu));
             // lds_slot(16 ks + 8 h + row, ch + 4 t) = (lds_slot(row, ch) ^ 64 t ^ 32 h) + (16 ks + 8 h) ROW
             int vat = (2 + buf) * TB + lds_slot<ROW>(4 * p + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 8 * (lane & 1);
             asm volatile("" : "+v"(vat));
