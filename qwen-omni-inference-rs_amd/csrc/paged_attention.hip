@@ -18,29 +18,31 @@ __global__ __launch_bounds__(JOIN_THREADS) void k_join(AttnArgs a) {
     const int tid = threadIdx.x, lane = tid % LANES, group = tid / LANES, sub = group % SUB;
     const int64_t item = (int64_t)blockIdx.x * (GROUPS / SUB) + group / SUB;
     const int row = (int)(item / a.heads), head = (int)(item - (int64_t)row * a.heads);
+    // The largest i < n with begin[i] <= x (ascending), -1: none.  A search with
+    // as many branches as the group has lanes.
+    auto last_from = [&](const int32_t* begin, int n, int x) {
+        int lo = -1, end = n - 1;  // between them, both included
+        while (lo < end) {
+            const int step = (end - lo + LANES - 1) / LANES, i = lo + (lane + 1) * step;
+            const uint64_t below = (__ballot(i <= end && begin[min(i, end)] <= x) >> (tid & 63 & ~(LANES - 1))) & (~0ull >> (64 - LANES));
+            lo += __popcll(below) * step;
+            end = min(end, lo + step - 1);
+        }
+        return lo;
+    };
     // the row's sequence, its prefix, and their pieces (none: own = pre = 0)
     int seq = row < a.batch.rows ? row : -1;
-    auto any_lane = [&](bool mine) {  // the lowest lane of the group that has it, -1
-        const uint64_t b = (__ballot(mine) >> (tid & 63 & ~(LANES - 1))) & (~0ull >> (64 - LANES));
-        return b ? __ffsll((unsigned long long)b) - 1 : -1;
-    };
-    if (a.batch.row_begin) {
-        int found = -1;
-        for (int s0 = 0; s0 < a.batch.batch; s0 += LANES) {
-            bool mine = false;
-            if (seq >= 0 && s0 + lane < a.batch.batch) {
-                const RowRange r = rows_of(a.batch, s0 + lane);
-                mine = row >= r.first && row - r.first < r.count;
-            }
-            const int w = any_lane(mine);
-            if (w >= 0 && found < 0) found = s0 + w;
+    if (a.batch.row_begin && seq >= 0) {
+        seq = last_from(a.batch.row_begin, a.batch.batch, row);
+        if (seq >= 0) {
+            const RowRange r = rows_of(a.batch, seq);
+            if (row < r.first || row - r.first >= r.count) seq = -1;
         }
-        seq = found;
     }
     int prefix = -1;
-    for (int g0 = 0; g0 < a.prefix.groups; g0 += LANES) {
-        const int w = any_lane(g0 + lane < a.prefix.groups && seq >= a.prefix.seq_begin[g0 + lane] && seq < a.prefix.seq_begin[g0 + lane + 1]);
-        if (w >= 0 && prefix < 0) prefix = g0 + w;
+    if (a.prefix.groups && seq >= 0) {
+        prefix = last_from(a.prefix.seq_begin, a.prefix.groups, seq);
+        if (prefix >= 0 && seq >= a.prefix.seq_begin[prefix + 1]) prefix = -1;
     }
     int own = 0, pre = 0;
     if (seq >= 0) {
@@ -139,9 +141,10 @@ struct Plan {
 // positions (PRE_FILL) leave these half the machine, and fewer pieces are less
 // to join: 64 rows behind 8192 positions 64, 45, 45, 49 and 59 us at 0.25, 0.5,
 // 0.75, 1 and 2.  Tiles alone: a chunk of f32 243, 222 and 233 us at 1, 2 and 4.
-// Few rows alone: 64 sequences of bf16 198, 198 and 193 us at 4, 8 and 16; with
-// a prefix the same 64 rows 45, 45, 45 and 48 us at 2, 4, 8 and 16.
-constexpr float FEW_FILL = 16, FEW_PRE_FILL = 4, TILE_FILL = 2, PRE_FILL = 0.5f;
+// Few rows alone: 64 sequences of bf16 198, 198, 193 and 211 us at 4, 8, 16 and
+// 32; with a prefix the 64 rows 45, 45, 45 and 48 us at 2, 4, 8 and 16, drafted
+// tokens of 11 sequences 17, 18, 18 and 18.
+constexpr float FEW_FILL = 16, FEW_PRE_FILL = 2, TILE_FILL = 2, PRE_FILL = 0.5f;
 
 size_t few_unit(bool f32_pages) { return f32_pages ? 64 : 128; }  // a tile for each of the four waves
 
