@@ -220,7 +220,9 @@ typedef struct {
  * past that are not worked on), max_pages table entries a sequence (positions
  * past them do not exist).  A table entry outside [0, num_pages) holds
  * nothing: its positions are not written and count as masked.  Rows from
- * row_begin[batch] on are left as they were. */
+ * row_begin[batch] on are left as they were.  Up to 65536 sequences, 2^23
+ * rows and 2^30 positions a sequence; up to 1024 kv heads and 16384 query
+ * heads. */
 typedef struct {
     uint32_t batch, rows, max_rows, max_pages;
     const int32_t* row_begin; /* [batch + 1], ascending, or null */
@@ -273,11 +275,15 @@ typedef struct {
  * the pages: the row at position p of its sequence sees positions 0 .. p.  A
  * row that sees nothing gives zeros; what a row does not see never reaches it,
  * whatever is stored there (NaN included).  Scores, maxima, sums and outputs
- * are held in 32 bits; between f32 rows and their pages products are as exact
- * as f32's, between bf16 ones the probabilities are rounded to bf16 before
- * they meet the values.  A row's result depends on its own sequence and the
- * sizes of the call, never on the other sequences.  Works in the context's
- * scratch buffer; enqueued without synchronizing. */
+ * are held in 32 bits.  f32 rows: products are as exact as float32's (q, the
+ * probabilities and f32 keys and values as sums of three bf16 terms; values
+ * below 2^-102 lose digits).  bf16 rows: the probabilities are rounded to bf16
+ * before they meet the values.  A row's result depends on its own sequence and
+ * the sizes of the call, never on the other sequences.  Rows of very different
+ * numbers a sequence (single tokens beside prompt chunks) are fastest in calls
+ * of their own.  rows * num_heads up to 2^23.  Works in the context's scratch
+ * buffer (lq8_paged_plan says how much of it); enqueued without synchronizing,
+ * apart from a call that has the buffer grow. */
 lq8_status lq8_paged_attention_device(lq8_ctx* ctx, const lq8_kv_pages* kv, const lq8_paged_batch* batch,
                                       const lq8_attn_rows* rows);
 
@@ -300,9 +306,9 @@ lq8_status lq8_prefix_attention_device(lq8_ctx* ctx, const lq8_kv_pages* kv, con
 /* Host-only: the checks of the two calls above (prefix null: the first), and
  * how they would run on num_workgroups compute units. */
 typedef struct {
-    uint32_t own_rows, own_splits;       /* rows (query row, head) a workgroup takes of a sequence; most pieces of its positions */
+    uint32_t own_rows, own_splits;       /* rows (query row, head) a workgroup takes, 16 or 128; most pieces of a sequence */
     uint32_t own_chunk;                  /* positions of the shortest piece */
-    uint32_t prefix_rows, prefix_splits, prefix_chunk;
+    uint32_t prefix_rows, prefix_splits, prefix_chunk; /* 0 without a prefix */
     uint64_t workgroups;                 /* of the launches together, the joining one aside */
     uint64_t scratch_bytes;              /* of the context's scratch buffer */
 } lq8_paged_info;

@@ -11,6 +11,12 @@
 // probabilities stay where they are, the maximum needs one exchange with lane
 // +- 32, and the rescaling of O none.  V is read transposed (ds_read_tr).
 // f32 rows: three bf16 terms of q and p each; f32 pages: of K and V too.
+//
+// Bound: the matrix cores are busy 37 % of the cycles, the vector instructions
+// 47 % (a bf16 chunk), and the two waves of a SIMD overlap them only in part.  Chunks of up to 2048 rows of three sequences over up to
+// 6100 positions, 32 heads over 8 of 128, bf16: 372 us, 880 TFLOP/s (a large
+// library product reaches 1204).  Tiles of 32 positions and three workgroups a
+// compute unit: 418 us; scores computed a tile ahead: no change.
 #pragma once
 
 #include <type_traits>

@@ -12,6 +12,11 @@
 // pairs into LDS, once for all heads, and go over the heads.  A thread has 2 V
 // elements of a head: V consecutive pairs, V = 16 bytes of elements, or 2 V of
 // what passes through; head_dim / (2 V) threads make a head.
+//
+// Bound: HBM for many rows, the launch for few.  4900 rows of 32 heads of 80,
+// two axes, bf16: 9.8 us, 5.1 TB/s read and written; the append of 7200 rows of
+// 32 + 2 x 8 heads of 128, bf16, with norms and three axes: 49 us, 4.0 TB/s; a
+// row of 24 heads 3.6 us.  (A 4 GiB copy reaches 4.8 TB/s.)
 #include <algorithm>
 #include <cmath>
 #include <new>
