@@ -316,7 +316,10 @@ __device__ __forceinline__ void tile_bf16_body(const AttnArgs& a, int block, cha
         }
         if (j < me.most) {
             v16f sc[SB];
+            // (ahead of the other wave's vector instructions: 369 us against 373)
+            __builtin_amdgcn_s_setprio(1);
             scores(buf * TB, sc);
+            __builtin_amdgcn_s_setprio(0);
             const bool masked = holes || j + N > me.least || !me.whole;
             // element e of block b: position 32 b + 8 (e / 4) + 4 p + e % 4
             float mx = -FLT_MAX;
@@ -579,6 +582,7 @@ __device__ __forceinline__ void tile_f32_body(const AttnArgs& a, int block, char
 #pragma unroll
                     for (int y = 0; y < 3; y++) ko[c % 2][y] = *(const v8b*)(sm + y * PB + (at ^ (c << 5)));
                 };
+                __builtin_amdgcn_s_setprio(1);  // (129 us against 138)
                 load_k(0);
 #pragma unroll
                 for (int e = 0; e < 16; e++) sc[e] = 0.0f;
@@ -595,6 +599,7 @@ __device__ __forceinline__ void tile_f32_body(const AttnArgs& a, int block, char
                     mul(sc, 0, 0);
                     __builtin_amdgcn_sched_barrier(0);
                 }
+                __builtin_amdgcn_s_setprio(0);
                 sc += lo;
             }
             const bool masked = pg[0] < 0 || pg[1] < 0 || j + N > me.least || !me.whole;
