@@ -141,28 +141,33 @@ struct Plan {
 // positions (PRE_FILL) leave these half the machine, and fewer pieces are less
 // to join: 64 rows behind 8192 positions 64, 45, 45, 49 and 59 us at 0.25, 0.5,
 // 0.75, 1 and 2.  Tiles alone: a chunk of f32 243, 222 and 233 us at 1, 2 and 4.
-// Few rows alone: 64 sequences of bf16 198, 198, 193 and 211 us at 4, 8, 16 and
-// 32; with a prefix the 64 rows 45, 45, 45 and 48 us at 2, 4, 8 and 16, drafted
-// tokens of 11 sequences 17, 18, 18 and 18.
-constexpr float FEW_FILL = 16, FEW_PRE_FILL = 2, TILE_FILL = 2, PRE_FILL = 0.5f;
+// Few rows: FEW_FILL, and more, up to FEW_MORE and 16 pieces, while a piece has
+// 512 positions for each row tile that reads them.  At 2, 4, 8 and 16 (bf16, 32
+// heads over 8 of 128):
+//     1 x 30000            27   30   38   38 us: short pieces, many to join
+//     8 x 4000             23   25   28   28
+//     24 x 9000            93   93   88   88: the pieces' ends even out
+//     64 x 8190           197  197  198  192
+constexpr float FEW_FILL = 2, FEW_MORE = 16, TILE_FILL = 2, PRE_FILL = 0.5f;
 
 size_t few_unit(bool f32_pages) { return f32_pages ? 64 : 128; }  // a tile for each of the four waves
 
 // Pieces of a part whose positions are at most `most`, in `groups` workgroups
 // a piece.  few: its kernel takes spans one by one, so that a long one among
-// short ones needs pieces of its own.
-Cut cut_of(size_t most, size_t groups, int cus, bool few, bool f32_pages, float fill) {
+// short ones needs pieces of its own; `tiles` row tiles read a span.
+Cut cut_of(size_t most, size_t groups, int cus, bool few, bool f32_pages, float tile_fill, size_t tiles) {
     Cut c;
     size_t pieces;
     if (few) {
         c.unit = few_unit(f32_pages);
         c.shortest = c.unit;
         const size_t longest = (most + 2047) / 2048, cap = 32768 / groups;
-        pieces = std::max((size_t)(fill * cus) / groups, std::min(longest, cap));
+        const size_t more = std::min<size_t>({(size_t)(FEW_MORE * cus) / groups, most / (512 * tiles), 16});
+        pieces = std::max<size_t>({(size_t)(FEW_FILL * cus) / groups, more, std::min(longest, cap)});
     } else {
         c.unit = f32_pages ? 32 : 64;
         c.shortest = 256;
-        pieces = (size_t)(fill * cus) / groups;
+        pieces = (size_t)(tile_fill * cus) / groups;
     }
     c.shift = __builtin_ctz(c.shortest);
     c.pieces = (int)std::max<size_t>(1, std::min(pieces, (most + c.shortest - 1) / c.shortest));
@@ -190,7 +195,7 @@ Plan plan_of(AttnArgs* a, PagedTypes types, int dim, int cus) {
     const size_t G = a->group, kvh = a->kv.kv_heads, rows = a->batch.rows, batch = a->batch.batch;
     const bool f32 = types == PT_F32_F32;
     // row tiles of `spans` spans that have `all` rows together, at most `most` each and `usual` by the rule's reckoning
-    auto part = [&](size_t spans, size_t all, size_t most, size_t usual, uint32_t pages, Cut* cut, int* few, bool* one, float few_fill, float tile_fill) {
+    auto part = [&](size_t spans, size_t all, size_t most, size_t usual, uint32_t pages, Cut* cut, int* few, bool* one, float tile_fill) {
         const size_t positions = (size_t)pages << a->kv.page_shift, units = (positions + few_unit(f32) - 1) / few_unit(f32);
         auto tiles_of = [&](size_t rows) {
             return std::min(spans * ((most * G + rows - 1) / rows), (all * G + (rows - 1) * std::min(spans, all)) / rows);
@@ -200,14 +205,14 @@ Plan plan_of(AttnArgs* a, PagedTypes types, int dim, int cus) {
         const bool is_few = takes_few(types, usual * G, tiles * kvh * units, cus);
         *few = is_few ? (int)tiles : 0;
         if (!is_few) tiles = tiles_of(TILE_PACKED);
-        *cut = cut_of(positions, tiles * kvh, cus, is_few, f32, is_few ? few_fill : tile_fill);
+        *cut = cut_of(positions, tiles * kvh, cus, is_few, f32, tile_fill, (usual * G + FEW_PACKED - 1) / FEW_PACKED);
         return tiles * kvh * cut->pieces;
     };
-    p.own_blocks = part(batch, rows, a->batch.max_rows, a->batch.max_rows, a->batch.max_pages, &a->own, &a->own_few, &a->own_each, a->prefix.groups ? FEW_PRE_FILL : FEW_FILL, TILE_FILL);
+    p.own_blocks = part(batch, rows, a->batch.max_rows, a->batch.max_rows, a->batch.max_pages, &a->own, &a->own_few, &a->own_each, TILE_FILL);
     p.slots = a->own.pieces;
     if (a->prefix.groups) {
         const size_t groups = a->prefix.groups;  // (each may have all rows)
-        p.pre_blocks = part(groups, rows, rows, (rows + groups - 1) / groups, a->prefix.max_pages, &a->pre, &a->pre_few, &a->pre_each, FEW_PRE_FILL, a->own_few ? PRE_FILL : TILE_FILL);
+        p.pre_blocks = part(groups, rows, rows, (rows + groups - 1) / groups, a->prefix.max_pages, &a->pre, &a->pre_few, &a->pre_each, a->own_few ? PRE_FILL : TILE_FILL);
         p.slots += a->pre.pieces;
     }
     if (p.slots > 1) p.scratch = p.slots * rows * a->heads * (dim * sizeof(float) + sizeof(float2));
