@@ -176,18 +176,22 @@ Cut cut_of(size_t most, size_t groups, int cus, bool few, bool f32_pages, float 
 
 // Row tiles of 16 fill their products but read the cache once each; tiles of
 // 128 read it once, with a workgroup's waves on 32 rows each (of few rows some
-// have none).  us, 16-row tiles / 128-row tiles, 32 heads over 8 of 128, 8 x
-// 4000 positions, by packed rows:
-//     packed                32            48            64            96
-//     bf16                  42 /  23      52 /  27      61 /  26      80 /  29
-//     f32 over bf16         42 /  37      47 /  45      57 /  45      69 /  48
-//     f32                   60 /  68      67 /  72      74 /  71     133 /  74
-// and 32 x 2000: f32 over bf16 55 / 64, 67 / 86, 82 / 86, 112 / 90; f32 87 /
-// 138, 116 / 160, 137 / 160, 243 / 168.  Where the blocks of 16 rows by a piece
-// are at most two a compute unit, latency decides: 1 x 2000 of bf16 11 / 15,
-// 13 / 17, 14 / 16 and (three a unit) 18 / 18.
+// have none).  us, 16-row tiles / 128-row tiles, 32 heads over 8 of 128, by
+// packed rows:
+//                  packed        32          48          64          96
+//     bf16           8 x  4000   37 /  23    55 /  27    60 /  26    56 /  29
+//                   32 x  2000   60 /  37    75 /  43    87 /  45   112 /  49
+//     f32 over bf16  8 x  4000   32 /  37    42 /  44    49 /  44    47 /  48
+//                   32 x  2000   49 /  64    55 /  85    66 /  85    85 /  90
+//                    1 x 30000   33 /  39    42 /  54    49 /  53    73 /  57
+//     f32            8 x  4000   59 /  64    94 /  73   103 /  71   128 /  74
+//                   32 x  2000   88 / 129   134 / 141   139 / 142   188 / 149
+//                    1 x 30000   57 /  71    81 /  79   101 /  82   159 /  94
+// Where the blocks of 16 rows by 128 positions are at most two a compute unit,
+// latency decides: 1 x 2000 of bf16 12 / 15, 14 / 17, 14 / 16; f32 15 / 35, 18 /
+// 38, 19 / 36.
 bool takes_few(PagedTypes types, size_t packed, size_t blocks, int cus) {
-    return packed <= (types == PT_BF16_BF16 ? 16 : types == PT_F32_BF16 ? 48 : 64) || blocks <= 2 * (size_t)cus;
+    return packed <= (types == PT_BF16_BF16 ? 16 : types == PT_F32_BF16 ? 64 : 32) || blocks <= 2 * (size_t)cus;
 }
 
 Plan plan_of(AttnArgs* a, PagedTypes types, int dim, int cus) {
@@ -196,7 +200,7 @@ Plan plan_of(AttnArgs* a, PagedTypes types, int dim, int cus) {
     const bool f32 = types == PT_F32_F32;
     // row tiles of `spans` spans that have `all` rows together, at most `most` each and `usual` by the rule's reckoning
     auto part = [&](size_t spans, size_t all, size_t most, size_t usual, uint32_t pages, Cut* cut, int* few, bool* one, float tile_fill) {
-        const size_t positions = (size_t)pages << a->kv.page_shift, units = (positions + few_unit(f32) - 1) / few_unit(f32);
+        const size_t positions = (size_t)pages << a->kv.page_shift, units = (positions + 127) / 128;
         auto tiles_of = [&](size_t rows) {
             return std::min(spans * ((most * G + rows - 1) / rows), (all * G + (rows - 1) * std::min(spans, all)) / rows);
         };

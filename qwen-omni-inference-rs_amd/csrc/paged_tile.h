@@ -14,7 +14,7 @@
 //
 // Bound: the matrix cores are busy 37 % of the cycles, the vector instructions
 // 47 % (a bf16 chunk), and the two waves of a SIMD overlap them only in part.  Chunks of up to 2048 rows of three sequences over up to
-// 6100 positions, 32 heads over 8 of 128, bf16: 372 us, 880 TFLOP/s (a large
+// 6100 positions, 32 heads over 8 of 128, bf16: 369 us, 890 TFLOP/s (a large
 // library product reaches 1204).  Tiles of 32 positions and three workgroups a
 // compute unit: 418 us; scores computed a tile ahead: no change.
 #pragma once
@@ -467,7 +467,7 @@ __device__ __forceinline__ void split_terms(v4f x0, v4f x1, v4u (&z)[3]) {
 
 // f32 pages.  The float32 products run at a sixteenth of the bf16 ones' rate,
 // so every operand is split into three bf16 terms, K and V on their way into
-// LDS, and the six products of terms that count are taken: 138 us for 951 rows
+// LDS, and the six products of terms that count are taken: 129 us for 951 rows
 // over 2999 positions, 16 heads over 8 of 128 (19.7 GFLOP), against 222 with
 // float32 products (152.8 TFLOP/s at most).  One tile in LDS, so that two
 // workgroups share a compute unit and one computes while the other splits.
