@@ -147,7 +147,7 @@ struct Plan {
 //     1 x 30000            27   30   38   38 us: short pieces, many to join
 //     8 x 4000             23   25   28   28
 //     24 x 9000            93   93   88   88: the pieces' ends even out
-//     64 x 8190           197  197  198  192
+//     64 x 8190           197  197  198  192 (191 with pieces of at least 512)
 constexpr float FEW_FILL = 2, FEW_MORE = 16, TILE_FILL = 2, PRE_FILL = 0.5f;
 
 size_t few_unit(bool f32_pages) { return f32_pages ? 64 : 128; }  // a tile for each of the four waves
@@ -160,8 +160,11 @@ Cut cut_of(size_t most, size_t groups, int cus, bool few, bool f32_pages, float 
     size_t pieces;
     if (few) {
         c.unit = few_unit(f32_pages);
-        c.shortest = c.unit;
-        const size_t longest = (most + 2047) / 2048, cap = 32768 / groups;
+        // (tables are often wider than their sequences: 64 of 1000 positions in
+        // tables for 131072 take 36 us, 34 in tables that fit; with pieces of a
+        // unit each and up to 32768 workgroups 71)
+        c.shortest = FEW_FILL * cus >= 8 * groups ? c.unit : 512;
+        const size_t longest = (most + 2047) / 2048, cap = 8192 / groups;
         const size_t more = std::min<size_t>({(size_t)(FEW_MORE * cus) / groups, most / (512 * tiles), 16});
         pieces = std::max<size_t>({(size_t)(FEW_FILL * cus) / groups, more, std::min(longest, cap)});
     } else {

@@ -6,7 +6,7 @@
 // f32: 16 KiB of K and V at head_dim 128), with no barrier before the end: the
 // next tile's K goes out when the scores are done and its V when this one's has
 // left its registers, so a wave always has about a tile in flight.  64 sequences
-// of up to 8190 bf16 positions, 32 heads over 8 of 128: 193 us, 5.76 TB/s (a
+// of up to 8190 bf16 positions, 32 heads over 8 of 128: 191 us, 5.83 TB/s (a
 // read-only stream reaches 6.8); f32 rows over 8 x 131072: 400 us, 5.3 TB/s (a
 // third workgroup on a compute unit would need its registers).
 //

@@ -49,7 +49,7 @@ def test_plans(seed):
         for name, positions, spans, most in parts:
             tile, splits, chunk = p[name + "_rows"], p[name + "_splits"], p[name + "_chunk"]
             assert tile in (16, 128)
-            assert chunk & (chunk - 1) == 0 and 64 <= chunk <= 256
+            assert chunk & (chunk - 1) == 0 and 64 <= chunk <= 512
             assert 1 <= splits <= -(-positions // chunk)
             # row tiles for every way of sharing the rows out
             full = min(spans * -(-most * G // tile), (c["total"] * G + (tile - 1) * min(spans, c["total"])) // tile)
